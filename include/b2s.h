@@ -58,8 +58,10 @@ typedef enum b2s_type {
     B2S_TYPE_F32 = 0,
     B2S_TYPE_I8 = 24,
     B2S_TYPE_I32 = 26,
+    B2S_TYPE_BF16 = 30,       /* ggml's id; activations of include/b2s_kv.h */
     B2S_TYPE_I2_S = 36,
-    B2S_TYPE_I2_S_R = 1036
+    B2S_TYPE_I2_S_R = 1036,
+    B2S_TYPE_F8_E4M3 = 1037   /* 8-bit float (4 exponent, 3 mantissa bits); cache codes of include/b2s_kv.h */
 } b2s_type;
 
 /* Mirrors the fields of ggml_tensor that an op reads: type, ne[4], nb[4], data. */
@@ -77,7 +79,8 @@ const char *b2s_last_error(void);
 /* B2S_OK if the current CUDA device is sm_100 (compute capability 10.0). */
 int b2s_device_check(void);
 /* Reads (and with clear != 0 resets) the device error word of the current device: bit 0 = a pipeline
- * wait timed out, bit 1 = a drain wait at kernel exit timed out. Synchronous. */
+ * wait timed out, bit 1 = a drain wait at kernel exit timed out, bit 2 = an index that a kernel read from
+ * device memory (a cache slot or page, a sequence's rows or length; include/b2s_kv.h) was out of range. Synchronous. */
 int b2s_device_error(uint32_t *out_bits, int clear);
 
 /* Test hook for the failure path of the kernels' bounded waits (no counterpart in the reference; failure

@@ -1,0 +1,271 @@
+// kv_api.cu -- the extern "C" boundary of include/b2s_kv.h: argument checks, workspace layout, dispatch.
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "b2s_internal.h"
+#include "b2s_kv.h"
+#include "kv_internal.h"
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return b2s::set_last_error(code, buf);
+}
+
+int launched(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return B2S_OK;
+    (void)cudaGetLastError();  // a failed launch must not leak into the next call's error check
+    return fail(B2S_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
+constexpr int64_t kMaxInt = 0x7fffffff;
+constexpr int kMaxBatch = 16384;
+
+int check_type(int32_t type, const char* op) {
+    if (type != B2S_TYPE_F32 && type != B2S_TYPE_BF16)
+        return fail(B2S_ERR_UNSUPPORTED, "%s: type %d is not f32 or bf16", op, (int)type);
+    return B2S_OK;
+}
+size_t size_of(int32_t type) { return type == B2S_TYPE_BF16 ? 2 : 4; }
+
+// M rows of `width` values of `type`, 16-byte aligned.
+int check_rows(const void* p, int64_t M, int64_t ld, int64_t width, int32_t type, const char* op, const char* name) {
+    if (M == 0) return B2S_OK;
+    if (!p) return fail(B2S_ERR_INVALID_ARG, "%s: %s is NULL", op, name);
+    if (ld < width) return fail(B2S_ERR_INVALID_ARG, "%s: %s rows of %lld values have stride %lld", op, name, (long long)width, (long long)ld);
+    if (!aligned(p, 16) || ld * (int64_t)size_of(type) % 16 != 0)
+        return fail(B2S_ERR_UNSUPPORTED, "%s: %s needs a 16-byte aligned base and a row stride that is a multiple of 16 bytes", op, name);
+    return B2S_OK;
+}
+
+int cache_view(const b2s_kv_cache* c, b2s::KvView* v, const char* op) {
+    if (!c) return fail(B2S_ERR_INVALID_ARG, "%s: cache is NULL", op);
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(B2S_ERR_INVALID_ARG, "%s: a cache buffer is NULL", op);
+    if (c->type != B2S_TYPE_I8 && c->type != B2S_TYPE_F8_E4M3)
+        return fail(B2S_ERR_UNSUPPORTED, "%s: cache type %d is not i8 or f8_e4m3", op, (int)c->type);
+    if (c->n_kv_heads <= 0 || c->head_dim <= 0 || c->n_pages <= 0 || c->page_size <= 0)
+        return fail(B2S_ERR_INVALID_ARG, "%s: cache has a non-positive dimension", op);
+    if (c->head_dim % 16 != 0 || c->head_dim > 128)
+        return fail(B2S_ERR_UNSUPPORTED, "%s: head_dim %d is not a multiple of 16 up to 128", op, c->head_dim);
+    if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return fail(B2S_ERR_UNSUPPORTED, "%s: page_size %d is not a power of two from 16 to 1024", op, c->page_size);
+    if (c->n_kv_heads > 4096 || c->n_pages > kMaxInt)
+        return fail(B2S_ERR_UNSUPPORTED, "%s: cache of %d heads and %lld pages is too large", op, c->n_kv_heads, (long long)c->n_pages);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
+        return fail(B2S_ERR_UNSUPPORTED, "%s: cache codes need 16-byte alignment, scales 4-byte", op);
+    v->k = static_cast<uint8_t*>(c->k);
+    v->v = static_cast<uint8_t*>(c->v);
+    v->ks = c->k_scale;
+    v->vs = c->v_scale;
+    v->n_pages = c->n_pages;
+    v->kv_heads = c->n_kv_heads;
+    v->hd = c->head_dim;
+    v->page_shift = __builtin_ctz((unsigned)c->page_size);
+    v->e4m3 = c->type == B2S_TYPE_F8_E4M3;
+    return B2S_OK;
+}
+
+// Workspace of an attention call: partial results, then the prefix's softmax states.
+struct AttnWs {
+    size_t part, m, l, o, total;
+    int pieces;
+};
+AttnWs attn_ws(int64_t M, int heads, int hd, int64_t prefix_len) {
+    AttnWs w;
+    w.part = 0;
+    w.m = a256(b2s::kv_attn_part_bytes());
+    w.pieces = prefix_len > 0 ? 1 : 0;
+    const size_t rows = (size_t)M * heads * w.pieces;
+    w.l = w.m + a256(rows * sizeof(float));
+    w.o = w.l + a256(rows * sizeof(float));
+    w.total = w.o + a256(rows * hd * sizeof(float));
+    return w;
+}
+
+int check_shapes(const b2s::KvView& v, const b2s_kv_batch* b, int64_t M, int n_heads, int64_t prefix_len, const char* op) {
+    if (!b) return fail(B2S_ERR_INVALID_ARG, "%s: batch is NULL", op);
+    if (b->batch < 0 || M < 0 || b->max_q < 0 || b->max_pages < 0 || prefix_len < 0)
+        return fail(B2S_ERR_INVALID_ARG, "%s: a size is negative", op);
+    if (n_heads <= 0 || n_heads % v.kv_heads != 0)
+        return fail(B2S_ERR_INVALID_ARG, "%s: %d query heads on %d key/value heads", op, n_heads, v.kv_heads);
+    if (b->batch > kMaxBatch) return fail(B2S_ERR_UNSUPPORTED, "%s: %d sequences, at most %d", op, b->batch, kMaxBatch);
+    const int64_t most = kMaxInt - 1024;
+    if (M > most / n_heads || b->max_pages > (most >> v.page_shift) || prefix_len > most)
+        return fail(B2S_ERR_UNSUPPORTED, "%s: rows x heads, tokens of a sequence and prefix_len have to be below 2^31", op);
+    return B2S_OK;
+}
+
+int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* batch, const int32_t* prefix_pages,
+              int64_t prefix_len, int32_t type, const void* q, int64_t ldq, int64_t M, int n_heads, float scale, int causal,
+              void* o, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    b2s::KvView v{};
+    int rc;
+    if ((rc = cache_view(cache, &v, op))) return rc;
+    if ((rc = check_type(type, op))) return rc;
+    if ((rc = check_shapes(v, batch, M, n_heads, prefix_len, op))) return rc;
+    const int64_t width = (int64_t)n_heads * v.hd;
+    if ((rc = check_rows(q, M, ldq, width, type, op, "q"))) return rc;
+    if ((rc = check_rows(o, M, ldo, width, type, op, "o"))) return rc;
+    if (!std::isfinite(scale)) return fail(B2S_ERR_INVALID_ARG, "%s: scale is not finite", op);
+    if (batch->batch > 0) {
+        if (!batch->q_start || !batch->kv_len) return fail(B2S_ERR_INVALID_ARG, "%s: q_start or kv_len is NULL", op);
+        if (batch->max_pages > 0 && !batch->pages) return fail(B2S_ERR_INVALID_ARG, "%s: pages is NULL", op);
+        if (batch->ld_pages < batch->max_pages) return fail(B2S_ERR_INVALID_ARG, "%s: ld_pages < max_pages", op);
+    }
+    if (prefix_len > 0 && !prefix_pages) return fail(B2S_ERR_INVALID_ARG, "%s: prefix_pages is NULL", op);
+    const AttnWs w = attn_ws(M, n_heads, v.hd, prefix_len);
+    if (!workspace || workspace_bytes < w.total)
+        return fail(B2S_ERR_WORKSPACE, "%s needs %zu workspace bytes, got %zu", op, w.total, workspace ? workspace_bytes : 0);
+    if (!aligned(workspace, 256)) return fail(B2S_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", op);
+    if ((rc = b2s_device_check())) return rc;
+    if (M == 0 || batch->batch == 0) return B2S_OK;
+
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    b2s::KvAttnArgs a{};
+    a.c = v;
+    a.q = q;
+    a.o = o;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.M = M;
+    a.heads = n_heads;
+    a.group = n_heads / v.kv_heads;
+    a.scale_log2e = scale * 1.4426950408889634f;
+    a.bf16 = type == B2S_TYPE_BF16;
+    a.part = reinterpret_cast<float*>(ws + w.part);
+    a.q_start = batch->q_start;
+    const b2s::AttnState state{reinterpret_cast<float*>(ws + w.m), reinterpret_cast<float*>(ws + w.l),
+                               reinterpret_cast<float*>(ws + w.o), w.pieces};
+    if (prefix_len > 0) {  // the batch's rows as one sequence over the prefix
+        b2s::KvAttnArgs p = a;
+        p.batch = 1;
+        p.q_stride = batch->batch;
+        p.kv_const = prefix_len;
+        p.pages = prefix_pages;
+        p.max_pages = (prefix_len + cache->page_size - 1) / cache->page_size;
+        p.to_state = true;
+        p.out = state;
+        if ((rc = launched(b2s::launch_kv_attention(p, st), op))) return rc;
+        a.add = state;
+    }
+    a.batch = batch->batch;
+    a.q_stride = 1;
+    a.kv_len = batch->kv_len;
+    a.pages = batch->pages;
+    a.ld_pages = batch->ld_pages;
+    a.max_pages = batch->max_pages;
+    a.causal = causal != 0;
+    return launched(b2s::launch_kv_attention(a, st), op);
+}
+
+}  // namespace
+
+extern "C" {
+
+int b2s_rope_axes(int32_t type, const void* x, int64_t ldx, int64_t M, int n_heads, int head_dim, const int32_t* pos,
+                  int64_t ldpos, int n_axes, const int32_t* sections, int interleaved, float theta_base, void* y,
+                  int64_t ldy, void* stream) {
+    int rc;
+    if ((rc = check_type(type, "rope_axes"))) return rc;
+    if (!sections || (M > 0 && (!x || !y || !pos)))
+        return fail(B2S_ERR_INVALID_ARG, "rope_axes: x, y, pos and sections must be non-NULL");
+    if (M < 0 || n_heads <= 0 || head_dim <= 0 || head_dim % 2) return fail(B2S_ERR_INVALID_ARG, "rope_axes: bad shape");
+    if (head_dim > 256 || n_heads > 65535 || M > kMaxInt)
+        return fail(B2S_ERR_UNSUPPORTED, "rope_axes: head_dim up to 256, n_heads up to 65535 and M below 2^31");
+    const int64_t width = (int64_t)n_heads * head_dim;
+    if (ldx < width || ldy < width) return fail(B2S_ERR_INVALID_ARG, "rope_axes: row stride below n_heads * head_dim");
+    if (!aligned(x, size_of(type)) || !aligned(y, size_of(type)))
+        return fail(B2S_ERR_UNSUPPORTED, "rope_axes: x or y is not aligned to its type");
+    if (M > 1 && x == y && ldx != ldy) return fail(B2S_ERR_INVALID_ARG, "rope_axes: in place needs ldx == ldy");
+    if (n_axes < 1 || n_axes > 4 || ldpos < n_axes) return fail(B2S_ERR_INVALID_ARG, "rope_axes: n_axes must be 1..4 and ldpos >= n_axes");
+    if (!(theta_base > 0.0f) || !std::isfinite(theta_base)) return fail(B2S_ERR_INVALID_ARG, "rope_axes: theta_base must be positive");
+    int64_t sum = 0;
+    for (int i = 0; i < n_axes; ++i) {
+        if (sections[i] < 0) return fail(B2S_ERR_INVALID_ARG, "rope_axes: a section is negative");
+        sum += sections[i];
+    }
+    if (sum != head_dim / 2)
+        return fail(B2S_ERR_INVALID_ARG, "rope_axes: sections add up to %lld, not to head_dim / 2 = %d", (long long)sum, head_dim / 2);
+    b2s::RopePairs p{};
+    const int half = head_dim / 2;
+    int left[4] = {0, 0, 0, 0};
+    for (int i = 0; i < n_axes; ++i) left[i] = sections[i];
+    for (int i = 0, ax = 0; i < half; ++i) {
+        while (left[ax] == 0) ax = (ax + 1) % n_axes;
+        p.axis[i] = (uint8_t)ax;
+        --left[ax];
+        if (interleaved) ax = (ax + 1) % n_axes;
+        p.turn[i] = std::pow((double)theta_base, -2.0 * i / head_dim) / 3.14159265358979323846;
+    }
+    if ((rc = b2s_device_check())) return rc;
+    return launched(b2s::launch_rope_axes(type == B2S_TYPE_BF16, x, ldx, M, n_heads, head_dim, pos, ldpos, p, y, ldy,
+                                          static_cast<cudaStream_t>(stream)),
+                    "rope_axes");
+}
+
+int b2s_kv_write(const b2s_kv_cache* cache, int32_t type, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                 int64_t M, const int64_t* slots, void* stream) {
+    b2s::KvView c{};
+    int rc;
+    if ((rc = cache_view(cache, &c, "kv_write"))) return rc;
+    if ((rc = check_type(type, "kv_write"))) return rc;
+    if (M < 0 || M > kMaxInt) return fail(B2S_ERR_INVALID_ARG, "kv_write: bad M");
+    if (M > 0 && !slots) return fail(B2S_ERR_INVALID_ARG, "kv_write: slots is NULL");
+    const int64_t width = (int64_t)c.kv_heads * c.hd;
+    if ((rc = check_rows(k, M, ldk, width, type, "kv_write", "k"))) return rc;
+    if ((rc = check_rows(v, M, ldv, width, type, "kv_write", "v"))) return rc;
+    if ((rc = b2s_device_check())) return rc;
+    return launched(b2s::launch_kv_write(c, type == B2S_TYPE_BF16, k, ldk, v, ldv, M, slots, static_cast<cudaStream_t>(stream)),
+                    "kv_write");
+}
+
+int b2s_kv_read(const b2s_kv_cache* cache, const int64_t* slots, int64_t M, int32_t type, void* k, int64_t ldk, void* v,
+                int64_t ldv, void* stream) {
+    b2s::KvView c{};
+    int rc;
+    if ((rc = cache_view(cache, &c, "kv_read"))) return rc;
+    if ((rc = check_type(type, "kv_read"))) return rc;
+    if (M < 0 || M > kMaxInt) return fail(B2S_ERR_INVALID_ARG, "kv_read: bad M");
+    if (M > 0 && !slots) return fail(B2S_ERR_INVALID_ARG, "kv_read: slots is NULL");
+    if (M > 0 && !k && !v) return fail(B2S_ERR_INVALID_ARG, "kv_read: k and v are both NULL");
+    const int64_t width = (int64_t)c.kv_heads * c.hd;
+    if (k && (rc = check_rows(k, M, ldk, width, type, "kv_read", "k"))) return rc;
+    if (v && (rc = check_rows(v, M, ldv, width, type, "kv_read", "v"))) return rc;
+    if ((rc = b2s_device_check())) return rc;
+    return launched(b2s::launch_kv_read(c, slots, M, type == B2S_TYPE_BF16, k, ldk, v, ldv, static_cast<cudaStream_t>(stream)),
+                    "kv_read");
+}
+
+size_t b2s_attention_kv_workspace_size(const b2s_kv_cache* cache, const b2s_kv_batch* batch, int64_t M, int n_heads,
+                                       int64_t prefix_len) {
+    b2s::KvView v{};
+    if (cache_view(cache, &v, "attention_kv_workspace_size")) return 0;
+    if (check_shapes(v, batch, M, n_heads, prefix_len, "attention_kv_workspace_size")) return 0;
+    return attn_ws(M, n_heads, v.hd, prefix_len).total;
+}
+
+int b2s_attention_kv(const b2s_kv_cache* cache, const b2s_kv_batch* batch, int32_t type, const void* q, int64_t ldq,
+                     int64_t M, int n_heads, float scale, int causal, void* o, int64_t ldo, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    return attention("attention_kv", cache, batch, nullptr, 0, type, q, ldq, M, n_heads, scale, causal, o, ldo, workspace,
+                     workspace_bytes, stream);
+}
+
+int b2s_attention_kv_prefix(const b2s_kv_cache* cache, const b2s_kv_batch* batch, const int32_t* prefix_pages,
+                            int64_t prefix_len, int32_t type, const void* q, int64_t ldq, int64_t M, int n_heads,
+                            float scale, int causal, void* o, int64_t ldo, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    return attention("attention_kv_prefix", cache, batch, prefix_pages, prefix_len, type, q, ldq, M, n_heads, scale, causal,
+                     o, ldo, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

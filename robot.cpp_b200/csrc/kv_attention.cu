@@ -1,0 +1,696 @@
+// kv_attention.cu -- attention of few query rows for each key/value head over the paged 8-bit cache: decoding steps,
+// drafts and short tails. One pass over the keys with the running maximum and sum of the softmax.
+//
+// Floor: the cache bytes, (2 hd + 8) per token and key/value head. A decoding step does 4 * group * hd operations on
+// them, so the products only have to keep up with memory.
+//
+// Products: warp-level fp16 MMAs, m16n8k16, fp32 accumulation. 8-bit codes (int8 and e4m3) are exact in fp16, so only
+// the fp32 side of a product is split: a query row, scaled by the power of two that brings its largest element to
+// 2^14, is hi + lo with hi = fp16(x), lo = fp16(x - hi) (relative error 2^-22; elements 2^-38 below the largest one
+// lose bits). The eight rows of a unit are MMA rows 0-7 as hi and 8-15 as lo: one MMA gives both parts and their sum
+// is in one thread. bf16 queries are exact in hi. Probabilities, times the value scale, are split alike.
+//   score(j) = (hi + lo)(q * scale * log2 e) . code(j) * k_scale(j);   p(j) = 2^(score - m);
+//   o = sum p(j) v_scale(j) code(j) / sum p(j)
+// The value scales are brought into fp16's range by a power of two above the largest one seen (vref).
+//
+// Split: a unit is (sequence, key/value head, eight query rows), its keys are tiles of 32. All units' tiles, laid end to
+// end, are cut into equal ranges, one for each resident block, so that uneven lengths load every SM alike. A block's
+// four warps take the tiles of its range in turn, each through its own ring of three asynchronous copies (no block-wide
+// wait between tiles, the ring runs on across units); at a unit's end they are joined through shared memory. A unit cut
+// by a range's border leaves partial results that kv_attention_join_kernel puts together: the order is fixed by the
+// lengths alone, so results do not change from run to run.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <atomic>
+
+#include "b2s_internal.h"
+#include "kv_internal.h"
+
+namespace b2s {
+
+namespace kva {
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kTile = 32;   // keys per warp step
+constexpr int kRows = 8;    // query rows of a unit
+constexpr int kStages = 3;
+constexpr int kMaxCtas = 320;
+constexpr int kMinTiles = 8;  // a block gets at least this many tiles (two steps of each warp)
+template <int HD>
+constexpr int kStageBytes = 2 * kTile * HD + 2 * kTile * 4 + 128;  // K, V codes, scales, flags
+template <int HD>
+constexpr int kPart = kRows * HD + 2 * kRows;  // floats of a partial result: o, m, l
+}  // namespace kva
+
+namespace {
+
+using namespace kva;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^e of a biased exponent 1..254.
+__device__ __forceinline__ float pow2_biased(int e) { return __int_as_float(e << 23); }
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
+    uint32_t d;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(d) : "r"(w));
+    return d;
+}
+// hi and lo fp16 parts of two values, packed (x0 in the low half).
+__device__ __forceinline__ void split_h2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(__fsub_rn(x0, f.x), __fsub_rn(x1, f.y));
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Two pairs of fp16 codes from two words of bytes whose 16-bit halves are {a0 a1}, {b0 b1} in x (e4m3: {a0 b0}, {a1 b1}).
+// int8: 1024 + (b + 128) is the fp16 number 0x6400 | (b ^ 0x80); 1152 is taken off again. Both steps are exact.
+template <bool E4M3>
+__device__ __forceinline__ void unpack4(uint32_t x, uint32_t& p0, uint32_t& p1) {
+    if (E4M3) {
+        p0 = e4m3x2_to_h2(x);
+        p1 = e4m3x2_to_h2(x >> 16);
+    } else {
+        p0 = sub_h2((x & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+        p1 = sub_h2(((x >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+    }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+    const int n = on ? 16 : 0;  // 0 bytes: nothing is read, zeros are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool on) {
+    const int n = on ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ---------------------------------------------------------------- units
+struct Seq {
+    int lo, n, len;    // first query row, query rows, keys
+    int row_tiles, units, tiles;
+};
+
+__device__ __forceinline__ Seq seq_of(const KvAttnArgs& a, int b) {
+    Seq s;
+    const int lo = a.q_start[b * a.q_stride], hi = a.q_start[(b + 1) * a.q_stride];
+    int64_t len = a.kv_len ? (int64_t)a.kv_len[b] : a.kv_const;
+    const int64_t cap = a.max_pages << a.c.page_shift;
+    bool bad = lo < 0 || hi < lo || hi > a.M;
+    s.lo = lo;
+    s.n = bad ? 0 : hi - lo;
+    if (len < 0 || len > cap) {
+        bad = true;
+        len = len < 0 ? 0 : cap;
+    }
+    if (bad) atomicOr(&g_device_error, kErrIndex);
+    s.len = (int)len;
+    s.row_tiles = (s.n * a.group + kRows - 1) / kRows;
+    s.units = s.row_tiles * a.c.kv_heads;
+    s.tiles = s.len > kTile ? (s.len + kTile - 1) / kTile : 1;
+    return s;
+}
+__device__ __forceinline__ int64_t work_of(const Seq& s) { return (int64_t)s.units * s.tiles; }
+
+struct Place {
+    int b;
+    int64_t off;  // tiles into the sequence's work
+};
+
+// Inclusive sum of v over the block's threads, and the block's total.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = v;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sh[w];
+        total += sh[w];
+    }
+    return v + before;
+}
+
+struct Ranges {
+    int64_t total;
+    int ctas;
+    __device__ __forceinline__ int64_t start(int c) const { return total * c / ctas; }
+};
+
+// All threads: the total of tiles, how many blocks share them, and the place of block c's first tile (c < ctas).
+__device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, Place& place, int64_t* sh, Place* sh_place) {
+    int64_t total = 0, w = 0, incl = 0, sum;
+    for (int base = 0; base < a.batch; base += kThreads) {
+        const int b = base + threadIdx.x;
+        w = b < a.batch ? work_of(seq_of(a, b)) : 0;
+        incl = block_scan(w, sh, sum);
+        total += sum;
+    }
+    Ranges r;
+    r.total = total;
+    const int64_t want = (total + kMinTiles - 1) / kMinTiles;
+    r.ctas = (int)(want < gridDim.x ? want : gridDim.x);
+    if (c >= r.ctas) return r;
+    const int64_t target = r.start(c);
+    if (a.batch <= kThreads) {
+        if (target >= incl - w && target < incl) *sh_place = Place{(int)threadIdx.x, target - (incl - w)};
+    } else {
+        int64_t before = 0;
+        for (int base = 0; base < a.batch; base += kThreads) {
+            const int b = base + threadIdx.x;
+            w = b < a.batch ? work_of(seq_of(a, b)) : 0;
+            incl = block_scan(w, sh, sum) + before;
+            if (target >= incl - w && target < incl) *sh_place = Place{b, target - (incl - w)};
+            before += sum;
+        }
+    }
+    __syncthreads();
+    place = *sh_place;
+    return r;
+}
+
+// A block's way through its range, one segment (a unit's tiles t0 .. t1 - 1) after another.
+struct Walk {
+    Seq s;
+    int b, u, t0, t1;
+    int64_t pos, end;
+    __device__ __forceinline__ void clip() { t1 = (int)min((int64_t)s.tiles, t0 + (end - pos)); }
+    __device__ __forceinline__ void begin(const KvAttnArgs& a, const Place& p, int64_t first, int64_t last) {
+        b = p.b;
+        s = seq_of(a, b);
+        pos = first;
+        end = last;
+        u = (int)(p.off / s.tiles);
+        t0 = (int)(p.off - (int64_t)u * s.tiles);
+        clip();
+    }
+    __device__ __forceinline__ bool done() const { return pos >= end; }
+    __device__ __forceinline__ void advance(const KvAttnArgs& a) {
+        pos += t1 - t0;
+        if (pos >= end) return;
+        if (++u == s.units) {
+            u = 0;
+            do {
+                s = seq_of(a, ++b);
+            } while (s.units == 0);
+        }
+        t0 = 0;
+        clip();
+    }
+};
+
+// ---------------------------------------------------------------- results
+// `n` consecutive output values of one row, d .. d + n - 1 (all inside hd): joined with the added pieces, then written.
+template <int N>
+__device__ __forceinline__ void finish(const KvAttnArgs& a, int64_t row, int head, int d, float m, float l, float (&o)[N]) {
+    for (int s = 0; s < a.add.pieces; ++s) {
+        const int64_t i = ((int64_t)s * a.M + row) * a.heads + head;
+        const float mi = a.add.m[i], li = a.add.l[i], mn = fmaxf(m, mi);
+        const float x = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, mn)), y = mi == -INFINITY ? 0.0f : ex2(__fsub_rn(mi, mn));
+        l = __fmaf_rn(l, x, __fmul_rn(li, y));
+        const float* p = a.add.o + i * a.c.hd + d;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + j);
+            o[j] = __fmaf_rn(o[j], x, __fmul_rn(v.x, y));
+            o[j + 1] = __fmaf_rn(o[j + 1], x, __fmul_rn(v.y, y));
+            o[j + 2] = __fmaf_rn(o[j + 2], x, __fmul_rn(v.z, y));
+            o[j + 3] = __fmaf_rn(o[j + 3], x, __fmul_rn(v.w, y));
+        }
+        m = mn;
+    }
+    if (a.to_state) {
+        const int64_t i = row * a.heads + head;
+        if (d == 0) {
+            a.out.m[i] = m;
+            a.out.l[i] = l;
+        }
+        float* p = a.out.o + i * a.c.hd + d;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = l == 0.0f ? 0.0f : __fmul_rn(o[j], inv);
+    const int64_t at = row * a.ldo + (int64_t)head * a.c.hd + d;
+    if (a.bf16) {
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(o[2 * j], o[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.o) + at;
+        if (N == 8)
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[N / 2 - 2], w[N / 2 - 1]);
+        else
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+        float* p = static_cast<float*>(a.o) + at;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+    }
+}
+
+// ---------------------------------------------------------------- the pass over the keys
+template <int HD, bool E4M3>
+__global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnArgs a) {
+    constexpr int kChunks = HD / 16;          // 16-byte chunks of a code row
+    constexpr int kStage = kStageBytes<HD>;
+    constexpr int kWords = HD / 16;           // 4-byte words of a thread's share of a key row (MMA k steps of scores)
+    constexpr int kVw = HD / 32;              // words of a thread's share of a value row
+    constexpr int kNt = HD / 8;               // output n tiles
+    constexpr int kOstride = HD / 4 + 4, kOrow = 4 * kOstride;  // padded output rows in shared memory (floats)
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int64_t sh_scan[kWarps];
+    __shared__ Place sh_place;
+    __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    griddep_wait();
+    griddep_launch();
+
+    Place place;
+    const Ranges rg = find_range(a, blockIdx.x, place, sh_scan, &sh_place);
+    if ((int)blockIdx.x >= rg.ctas) return;
+    const int64_t first = rg.start(blockIdx.x), last = rg.start(blockIdx.x + 1);
+    uint8_t* ring = smem + warp * (kStages * kStage);
+    const uint32_t ring_u = smem_u32(ring);
+
+    Walk cw;
+    cw.begin(a, place, first, last);
+
+    // ---- loader: the warp's tiles in order, one ahead with the page numbers
+    Walk lw = cw;
+    int lt = lw.t0 + warp;
+    int page_a = 0, page_b = 0;
+    bool have = true;
+    auto fetch = [&]() {  // the next tile of this warp, and the pages of its two halves
+        while (lt >= lw.t1) {
+            lw.advance(a);
+            if (lw.done()) {
+                have = false;
+                return;
+            }
+            lt = lw.t0 + warp;
+        }
+        const int k0 = lt * kTile;
+        const int32_t* pg = a.pages + (int64_t)lw.b * a.ld_pages;
+        page_a = k0 < lw.s.len ? pg[k0 >> a.c.page_shift] : 0;
+        page_b = k0 + 16 < lw.s.len ? pg[(k0 + 16) >> a.c.page_shift] : 0;
+    };
+    auto issue = [&](int stage) {
+        if (have) {
+            const uint32_t st = ring_u + stage * kStage;
+            const int k0 = lt * kTile, len = lw.s.len, mask = (1 << a.c.page_shift) - 1;
+            const int h = lw.u / lw.s.row_tiles;
+            const bool ok_a = page_a >= 0 && page_a < a.c.n_pages, ok_b = page_b >= 0 && page_b < a.c.n_pages;
+            if (!(ok_a && ok_b) && lane == 0) atomicOr(&g_device_error, kErrIndex);
+            // cache rows of keys k0 and k0 + 16
+            const int64_t ra = (((int64_t)page_a * a.c.kv_heads + h) << a.c.page_shift) + (k0 & mask);
+            const int64_t rb = (((int64_t)page_b * a.c.kv_heads + h) << a.c.page_shift) + ((k0 + 16) & mask);
+#pragma unroll
+            for (int p = 0; p < kTile * kChunks / 32; ++p) {
+                const int e = p * 32 + lane, r = e / kChunks, c = e % kChunks;
+                const bool on = (r < 16 ? ok_a : ok_b) && k0 + r < len && c * 16 < a.c.hd;
+                const int64_t off = on ? (r < 16 ? ra + r : rb + r - 16) * a.c.hd + c * 16 : 0;
+                const int f = HD == 128 ? (r & 7) : ((r >> 1) & 3);
+                const uint32_t dst = st + r * HD + ((c ^ f) << 4);
+                cp_async16(dst, a.c.k + off, on);
+                cp_async16(dst + kTile * HD, a.c.v + off, on);
+            }
+            const bool on = (lane < 16 ? ok_a : ok_b) && k0 + lane < len;
+            const int64_t row = on ? (lane < 16 ? ra + lane : rb + lane - 16) : 0;
+            cp_async4(st + 2 * kTile * HD + lane * 4, a.c.ks + row, on);
+            cp_async4(st + 2 * kTile * HD + kTile * 4 + lane * 4, a.c.vs + row, on);
+            if (lane == 0)
+                *reinterpret_cast<int*>(ring + stage * kStage + 2 * kTile * HD + 2 * kTile * 4) = (ok_a ? 1 : 0) | (ok_b ? 2 : 0);
+            lt += kWarps;
+            fetch();
+        }
+        cp_commit();
+    };
+    fetch();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
+    int it = 0;  // tiles this warp has taken
+
+    for (bool head_seg = true; !cw.done(); cw.advance(a), head_seg = false) {
+        const int h = cw.u / cw.s.row_tiles, row0 = (cw.u - h * cw.s.row_tiles) * kRows;
+        const int rows = min(kRows, cw.s.n * a.group - row0);
+        // ---- the query row of this thread's group, as MMA fragments: k step w holds hd values 4 w' .. 4 w' + 3 of
+        // the thread's contiguous share [t * HD / 4, (t + 1) * HD / 4)
+        uint32_t qh[kWords][2], ql[kWords][2];
+        float rf = 0.0f;  // takes scores back to log2 units
+        int limit = 0;    // keys that the row sees
+        {
+            float x[HD / 4];
+#pragma unroll
+            for (int i = 0; i < HD / 4; ++i) x[i] = 0.0f;
+            if (g < rows) {
+                const int r = row0 + g, i = r / a.group, head = h * a.group + (r - i * a.group);
+                limit = a.causal ? cw.s.len - cw.s.n + i + 1 : cw.s.len;
+                const int64_t at = (cw.s.lo + (int64_t)i) * a.ldq + (int64_t)head * a.c.hd + t * (HD / 4);
+#pragma unroll
+                for (int j = 0; j < HD / 4; j += 8) {
+                    if (t * (HD / 4) + j < a.c.hd) {
+                        if (a.bf16) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at + j);
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                x[j + 2 * k] = __uint_as_float(w[k] << 16);
+                                x[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                            }
+                        } else {
+                            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + j);
+                            const float4 u = p[0], w = p[1];
+                            x[j] = u.x, x[j + 1] = u.y, x[j + 2] = u.z, x[j + 3] = u.w;
+                            x[j + 4] = w.x, x[j + 5] = w.y, x[j + 6] = w.z, x[j + 7] = w.w;
+                        }
+                    }
+                }
+            }
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 4; ++i) big = fmaxf(big, fabsf(x[i]));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            // the row's largest element goes to [2^14, 2^15)
+            const int up = min(253, 268 - (__float_as_int(big) >> 23));
+            const float mul = pow2_biased(up);
+            rf = __fmul_rn(pow2_biased(254 - up), a.scale_log2e);
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+                float y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = __fmul_rn(x[4 * w + k], mul);
+                // int8 words unpack to bytes (0, 2) and (1, 3), e4m3 words to (0, 1) and (2, 3)
+                split_h2(y[0], E4M3 ? y[1] : y[2], qh[w][0], ql[w][0]);
+                split_h2(E4M3 ? y[2] : y[1], y[3], qh[w][1], ql[w][1]);
+            }
+        }
+        float oacc[kNt][4];
+#pragma unroll
+        for (int n = 0; n < kNt; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) oacc[n][k] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        int vref = 15;  // biased exponent above every value scale so far
+
+        for (int tile = cw.t0 + warp; tile < cw.t1; tile += kWarps, ++it) {
+            cp_wait<kStages - 2>();
+            __syncwarp();
+            issue((it + kStages - 1) % kStages);
+            const uint8_t* st = ring + (it % kStages) * kStage;
+            const float* ks = reinterpret_cast<const float*>(st + 2 * kTile * HD);
+            const float* vs = ks + kTile;
+            const int flags = *reinterpret_cast<const int*>(vs + kTile);
+            // ---- scores of 32 keys: thread (g, t) gets keys 8 n + 2 t, 8 n + 2 t + 1 of row g
+            float s[4][2];
+            float mx = -INFINITY, vmax = 0.0f;
+            float2 vsc[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                const int r = n * 8 + g;
+                const uint8_t* kr = st + r * HD;
+#pragma unroll
+                for (int half = 0; half < kWords / 4; ++half) {
+                    const int ch = HD == 128 ? (2 * t + half) ^ (r & 7) : t ^ ((r >> 1) & 3);
+                    const uint4 u = *reinterpret_cast<const uint4*>(kr + (ch << 4));
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t b0, b1;
+                        unpack4<E4M3>(w[k], b0, b1);
+                        mma_f16(c, qh[4 * half + k][0], ql[4 * half + k][0], qh[4 * half + k][1], ql[4 * half + k][1], b0, b1);
+                    }
+                }
+                const float2 f = *reinterpret_cast<const float2*>(ks + n * 8 + 2 * t);
+                vsc[n] = *reinterpret_cast<const float2*>(vs + n * 8 + 2 * t);
+                const int key = tile * kTile + n * 8 + 2 * t;
+                const bool there = (flags >> (n >> 1)) & 1;
+                const bool see0 = there && key < limit, see1 = there && key + 1 < limit;
+                s[n][0] = see0 ? __fmul_rn(__fmul_rn(__fadd_rn(c[0], c[2]), f.x), rf) : -INFINITY;
+                s[n][1] = see1 ? __fmul_rn(__fmul_rn(__fadd_rn(c[1], c[3]), f.y), rf) : -INFINITY;
+                mx = fmaxf(mx, fmaxf(s[n][0], s[n][1]));
+                // a value scale that a row does not see may be anything
+                vsc[n].x = see0 ? vsc[n].x : 0.0f;
+                vsc[n].y = see1 ? vsc[n].y : 0.0f;
+                vmax = fmaxf(vmax, fmaxf(fabsf(vsc[n].x), fabsf(vsc[n].y)));
+            }
+#pragma unroll
+            for (int o = 1; o <= 2; o <<= 1) {  // a row's keys are spread over four lanes
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+            }
+            // ---- running maximum, and the references that the outputs are kept in
+            const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.0f : mn;
+            float alpha = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, mu));
+            l = __fmul_rn(l, alpha);
+            const int e = __float_as_int(vmax) >> 23;
+            bool move = mn != m;
+            if (e >= vref) {  // the same in the row's four lanes
+                const int nref = min(e + 1, 255);
+                alpha = __fmul_rn(alpha, nref - vref > 126 ? 0.0f : pow2_biased(127 - (nref - vref)));
+                vref = nref;
+                move = true;
+            }
+            m = mn;
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) oacc[n][k] = __fmul_rn(oacc[n][k], alpha);
+            }
+            const float vmul = pow2_biased(268 - vref);
+            // ---- probabilities as the A fragments of two 16-key steps
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float p0 = ex2(__fsub_rn(s[n][0], mu)), p1 = ex2(__fsub_rn(s[n][1], mu));
+                l = __fadd_rn(l, __fadd_rn(p0, p1));
+                split_h2(__fmul_rn(p0, __fmul_rn(vsc[n].x, vmul)), __fmul_rn(p1, __fmul_rn(vsc[n].y, vmul)), ph[n], pl[n]);
+            }
+            // ---- outputs: n tile j holds hd columns g' * kNt + j
+            const uint8_t* vt = st + kTile * HD;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t w[4][kVw];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = j * 16 + 2 * t + (k & 1) + 8 * (k >> 1);
+                    if (HD == 128) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(vt + r * HD + ((g ^ (r & 7)) << 4));
+                        w[k][0] = u.x, w[k][1] = u.y, w[k][kVw - 2] = u.z, w[k][kVw - 1] = u.w;
+                    } else {
+                        const uint2 u =
+                            *reinterpret_cast<const uint2*>(vt + r * HD + (((g >> 1) ^ ((r >> 1) & 3)) << 4) + (g & 1) * 8);
+                        w[k][0] = u.x, w[k][1] = u.y;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < kVw; ++q) {
+                    uint32_t b0[4], b1[4];  // pairs (key 2t, key 2t + 1) and (key 2t + 8, key 2t + 9) of four columns
+                    constexpr uint32_t kLo = E4M3 ? 0x5140 : 0x5410, kHi = E4M3 ? 0x7362 : 0x7632;
+                    unpack4<E4M3>(__byte_perm(w[0][q], w[1][q], kLo), b0[0], b0[1]);
+                    unpack4<E4M3>(__byte_perm(w[0][q], w[1][q], kHi), b0[2], b0[3]);
+                    unpack4<E4M3>(__byte_perm(w[2][q], w[3][q], kLo), b1[0], b1[1]);
+                    unpack4<E4M3>(__byte_perm(w[2][q], w[3][q], kHi), b1[2], b1[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16(oacc[4 * q + k], ph[2 * j], pl[2 * j], ph[2 * j + 1], pl[2 * j + 1], b0[k], b1[k]);
+                }
+            }
+        }
+
+        // ---- join the four warps: every warp's free ring stage holds its outputs (the stage that its next copy fills)
+        l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 1));
+        l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 2));
+        if (t == 0) {
+            sh_m[warp][g] = m;
+            sh_l[warp][g] = l;
+        }
+        const int free_stage = (it + kStages - 1) % kStages;
+        __syncwarp();
+        {
+            const float back = pow2_biased(vref - 14);
+            float* ob = reinterpret_cast<float*>(ring + free_stage * kStage) + g * kOrow + t * kOstride;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int n = 0; n < kNt; n += 4) {
+                    float4 x;
+                    float* xp = &x.x;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        xp[k] = __fmul_rn(__fadd_rn(oacc[n + k][half], oacc[n + k][2 + half]), back);
+                    *reinterpret_cast<float4*>(ob + half * kNt + n) = x;
+                }
+        }
+        __shared__ int sh_free[kWarps];
+        if (lane == 0) sh_free[warp] = free_stage;
+        __syncthreads();
+        {
+            constexpr int N = HD / 16;
+            const int row = threadIdx.x / 16, d = (threadIdx.x % 16) * N;
+            float mm = -INFINITY, ll = 0.0f, o[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_m[w][row]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float mw = sh_m[w][row], f = mw == -INFINITY ? 0.0f : ex2(__fsub_rn(mw, mm));
+                const float* ob = reinterpret_cast<const float*>(smem + (w * kStages + sh_free[w]) * kStage) + row * kOrow +
+                                  (d / (HD / 4)) * kOstride + d % (HD / 4);
+                ll = __fmaf_rn(sh_l[w][row], f, ll);
+#pragma unroll
+                for (int j = 0; j < N; ++j) o[j] = __fmaf_rn(ob[j], f, o[j]);
+            }
+            if (cw.t0 == 0 && cw.t1 == cw.s.tiles) {
+                if (row < rows && d < a.c.hd) {
+                    const int r = row0 + row, i = r / a.group;
+                    finish<N>(a, cw.s.lo + (int64_t)i, h * a.group + (r - i * a.group), d, mm, ll, o);
+                }
+            } else {  // the first segment goes to slot 0, the last one to slot 1: no other can be cut
+                float* p = a.part + ((int64_t)blockIdx.x * 2 + (head_seg ? 0 : 1)) * kPart<HD>;
+#pragma unroll
+                for (int j = 0; j < N; j += 4)
+                    *reinterpret_cast<float4*>(p + row * HD + d + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                if (d == 0) {
+                    p[kRows * HD + row] = mm;
+                    p[kRows * HD + kRows + row] = ll;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    cp_wait<0>();
+}
+
+// Joins the partial results of every unit that the borders between blocks cut. Block c - 1 looks at border c and acts if
+// it is the first one inside its unit.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(const KvAttnArgs a) {
+    __shared__ int64_t sh_scan[kWarps];
+    __shared__ Place sh_place;
+    griddep_wait();
+    griddep_launch();
+    const int c = blockIdx.x;
+    Place place;
+    const Ranges rg = find_range(a, c, place, sh_scan, &sh_place);
+    if (c == 0 || c >= rg.ctas) return;
+    const Seq s = seq_of(a, place.b);
+    const int u = (int)(place.off / s.tiles), t = (int)(place.off - (int64_t)u * s.tiles);
+    const int64_t unit = rg.start(c) - t;
+    if (t == 0 || rg.start(c - 1) > unit) return;
+    const int h = u / s.row_tiles, row0 = (u - h * s.row_tiles) * kRows;
+    constexpr int N = HD / 16;
+    const int row = threadIdx.x / 16, d = (threadIdx.x % 16) * N;
+    int end = c + 1;
+    while (end < rg.ctas && rg.start(end) < unit + s.tiles) ++end;
+    auto piece = [&](int k) -> const float* {  // pieces of blocks c - 1 .. end - 1
+        return a.part + ((int64_t)k * 2 + (k == c - 1 && rg.start(c - 1) < unit ? 1 : 0)) * kPart<HD>;
+    };
+    float m = -INFINITY, l = 0.0f, o[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = 0.0f;
+    for (int k = c - 1; k < end; ++k) m = fmaxf(m, piece(k)[kRows * HD + row]);
+    for (int k = c - 1; k < end; ++k) {
+        const float* p = piece(k);
+        const float mk = p[kRows * HD + row], f = mk == -INFINITY ? 0.0f : ex2(__fsub_rn(mk, m));
+        l = __fmaf_rn(p[kRows * HD + kRows + row], f, l);
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + row * HD + d + j);
+            o[j] = __fmaf_rn(v.x, f, o[j]);
+            o[j + 1] = __fmaf_rn(v.y, f, o[j + 1]);
+            o[j + 2] = __fmaf_rn(v.z, f, o[j + 2]);
+            o[j + 3] = __fmaf_rn(v.w, f, o[j + 3]);
+        }
+    }
+    if (row < min(kRows, s.n * a.group - row0) && d < a.c.hd) {
+        const int r = row0 + row, i = r / a.group;
+        finish<N>(a, s.lo + (int64_t)i, h * a.group + (r - i * a.group), d, m, l, o);
+    }
+}
+
+int resident_blocks() {
+    static std::atomic<int> cache[128];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return 2 * 148;
+    if (!cache[dev]) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+        cache[dev] = 2 * n < kMaxCtas ? 2 * n : kMaxCtas;
+    }
+    return cache[dev];
+}
+
+template <typename K>
+cudaError_t launch_args(K kernel, int grid, size_t smem, const KvAttnArgs& a, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int HD, bool E4M3>
+cudaError_t launch_typed(const KvAttnArgs& a, cudaStream_t st) {
+    const size_t smem = (size_t)kWarps * kStages * kStageBytes<HD>;
+    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kv_attention_kernel<HD, E4M3>), smem);
+    if (e != cudaSuccess) return e;
+    const int grid = resident_blocks();
+    if ((e = launch_args(kv_attention_kernel<HD, E4M3>, grid, smem, a, st)) != cudaSuccess) return e;
+    return launch_args(kv_attention_join_kernel<HD>, grid, 0, a, st);
+}
+
+}  // namespace
+
+size_t kv_attn_part_bytes() { return sizeof(float) * 2 * kMaxCtas * kPart<128>; }
+
+cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st) {
+    if (a.batch <= 0 || a.M <= 0) return cudaSuccess;
+    if (a.c.hd > 64) return a.c.e4m3 ? launch_typed<128, true>(a, st) : launch_typed<128, false>(a, st);
+    return a.c.e4m3 ? launch_typed<64, true>(a, st) : launch_typed<64, false>(a, st);
+}
+
+}  // namespace b2s
