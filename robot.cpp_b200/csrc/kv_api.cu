@@ -1,4 +1,5 @@
 // kv_api.cu -- the extern "C" boundary of include/b2s_kv.h: argument checks, workspace layout, dispatch.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -73,20 +74,59 @@ int cache_view(const b2s_kv_cache* c, b2s::KvView* v, const char* op) {
     return B2S_OK;
 }
 
-// Workspace of an attention call: partial results, then the prefix's softmax states.
-struct AttnWs {
-    size_t part, m, l, o, total;
+// Which kernels take the rows of a call, decided from sizes that the host has. Sequences with at most kFewRows rows a
+// key/value head go to the warp-level kernel, which reads their keys once per eight rows; the others to the tensor-core
+// kernel, which reads them once per 128.
+constexpr int kFewRows = 64;
+struct Plan {
+    bool few, many;
+    int min_rows, splits;
+};
+Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys) {
+    Plan p{true, false, 0, 1};
+    if (max_q * group <= kFewRows) return p;
+    p.many = true;
+    p.few = M != batch * max_q;  // equal: every sequence has max_q rows
+    p.min_rows = p.few ? kFewRows : 0;
+    // Less than a wave of 128-row blocks: cut the keys, so that waves x (tiles of 128 keys + about four tiles' worth of
+    // starting and ending a block) is least.
+    const int64_t units = std::max<int64_t>(1, M * group / 128) * kv_heads, tiles = (keys + 127) / 128;
+    int64_t best = 0;
+    for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles) && units < 148; ++s) {
+        const int64_t cost = (units * s + 147) / 148 * ((tiles + s - 1) / s + 4) + (s > 1 ? 3 : 0);
+        if (s == 1 || cost < best) {
+            best = cost;
+            p.splits = s;
+        }
+    }
+    return p;
+}
+
+// Workspace of an attention call: partial results, then the softmax states of the own tokens' and the prefix's pieces.
+struct StateWs {
+    size_t m, l, o;
     int pieces;
 };
-AttnWs attn_ws(int64_t M, int heads, int hd, int64_t prefix_len) {
+struct AttnWs {
+    size_t part, total;
+    StateWs own, prefix;
+};
+AttnWs attn_ws(const Plan& own, const Plan& pre, int64_t M, int heads, int hd, int64_t prefix_len) {
     AttnWs w;
     w.part = 0;
-    w.m = a256(b2s::kv_attn_part_bytes());
-    w.pieces = prefix_len > 0 ? 1 : 0;
-    const size_t rows = (size_t)M * heads * w.pieces;
-    w.l = w.m + a256(rows * sizeof(float));
-    w.o = w.l + a256(rows * sizeof(float));
-    w.total = w.o + a256(rows * hd * sizeof(float));
+    w.total = a256(b2s::kv_attn_part_bytes());
+    auto take = [&](int pieces) {
+        const size_t rows = (size_t)M * heads * pieces;
+        StateWs s;
+        s.pieces = pieces;
+        s.m = w.total;
+        s.l = s.m + a256(rows * sizeof(float));
+        s.o = s.l + a256(rows * sizeof(float));
+        w.total = s.o + a256(rows * hd * sizeof(float));
+        return s;
+    };
+    w.own = take(own.many && (own.splits > 1 || prefix_len > 0) ? own.splits : 0);
+    w.prefix = take(prefix_len > 0 ? (pre.many ? pre.splits : 1) : 0);
     return w;
 }
 
@@ -121,7 +161,10 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
         if (batch->ld_pages < batch->max_pages) return fail(B2S_ERR_INVALID_ARG, "%s: ld_pages < max_pages", op);
     }
     if (prefix_len > 0 && !prefix_pages) return fail(B2S_ERR_INVALID_ARG, "%s: prefix_pages is NULL", op);
-    const AttnWs w = attn_ws(M, n_heads, v.hd, prefix_len);
+    const int group = n_heads / v.kv_heads;
+    const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift);
+    const Plan pre = plan_rows(M, 1, M, group, v.kv_heads, prefix_len);
+    const AttnWs w = attn_ws(own, pre, M, n_heads, v.hd, prefix_len);
     if (!workspace || workspace_bytes < w.total)
         return fail(B2S_ERR_WORKSPACE, "%s needs %zu workspace bytes, got %zu", op, w.total, workspace ? workspace_bytes : 0);
     if (!aligned(workspace, 256)) return fail(B2S_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", op);
@@ -138,13 +181,15 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     a.ldo = ldo;
     a.M = M;
     a.heads = n_heads;
-    a.group = n_heads / v.kv_heads;
+    a.group = group;
     a.scale_log2e = scale * 1.4426950408889634f;
     a.bf16 = type == B2S_TYPE_BF16;
     a.part = reinterpret_cast<float*>(ws + w.part);
     a.q_start = batch->q_start;
-    const b2s::AttnState state{reinterpret_cast<float*>(ws + w.m), reinterpret_cast<float*>(ws + w.l),
-                               reinterpret_cast<float*>(ws + w.o), w.pieces};
+    auto state = [&](const StateWs& s) {
+        return b2s::AttnState{reinterpret_cast<float*>(ws + s.m), reinterpret_cast<float*>(ws + s.l),
+                              reinterpret_cast<float*>(ws + s.o), s.pieces};
+    };
     if (prefix_len > 0) {  // the batch's rows as one sequence over the prefix
         b2s::KvAttnArgs p = a;
         p.batch = 1;
@@ -152,10 +197,12 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
         p.kv_const = prefix_len;
         p.pages = prefix_pages;
         p.max_pages = (prefix_len + cache->page_size - 1) / cache->page_size;
+        p.max_rows = (int)kMaxInt;
         p.to_state = true;
-        p.out = state;
-        if ((rc = launched(b2s::launch_kv_attention(p, st), op))) return rc;
-        a.add = state;
+        p.out = state(w.prefix);
+        rc = launched(pre.many ? b2s::launch_kv_attention_tc(p, pre.splits, st) : b2s::launch_kv_attention(p, st), op);
+        if (rc) return rc;
+        a.add = p.out;
     }
     a.batch = batch->batch;
     a.q_stride = 1;
@@ -164,6 +211,16 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     a.ld_pages = batch->ld_pages;
     a.max_pages = batch->max_pages;
     a.causal = causal != 0;
+    if (own.many) {
+        b2s::KvAttnArgs t = a;
+        t.min_rows = own.min_rows;
+        t.out = state(w.own);
+        t.to_state = w.own.pieces > 0;
+        if ((rc = launched(b2s::launch_kv_attention_tc(t, own.splits, st), op))) return rc;
+        if (t.to_state && (rc = launched(b2s::launch_kv_state_join(t, st), op))) return rc;
+    }
+    if (!own.few) return B2S_OK;
+    a.max_rows = own.many ? kFewRows : (int)kMaxInt;
     return launched(b2s::launch_kv_attention(a, st), op);
 }
 
@@ -250,7 +307,10 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache* cache, const b2s_kv_b
     b2s::KvView v{};
     if (cache_view(cache, &v, "attention_kv_workspace_size")) return 0;
     if (check_shapes(v, batch, M, n_heads, prefix_len, "attention_kv_workspace_size")) return 0;
-    return attn_ws(M, n_heads, v.hd, prefix_len).total;
+    const int group = n_heads / v.kv_heads;
+    return attn_ws(plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift),
+                   plan_rows(M, 1, M, group, v.kv_heads, prefix_len), M, n_heads, v.hd, prefix_len)
+        .total;
 }
 
 int b2s_attention_kv(const b2s_kv_cache* cache, const b2s_kv_batch* batch, int32_t type, const void* q, int64_t ldq,

@@ -127,7 +127,8 @@ __device__ __forceinline__ Seq seq_of(const KvAttnArgs& a, int b) {
     }
     if (bad) atomicOr(&g_device_error, kErrIndex);
     s.len = (int)len;
-    s.row_tiles = (s.n * a.group + kRows - 1) / kRows;
+    const int rows = s.n * a.group;
+    s.row_tiles = rows > a.min_rows && rows <= a.max_rows ? (rows + kRows - 1) / kRows : 0;
     s.units = s.row_tiles * a.c.kv_heads;
     s.tiles = s.len > kTile ? (s.len + kTile - 1) / kTile : 1;
     return s;

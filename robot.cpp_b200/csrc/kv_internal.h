@@ -53,16 +53,24 @@ struct KvAttnArgs {
     const int32_t* pages;
     int64_t ld_pages, max_pages;
     int batch, heads, group;
+    int min_rows, max_rows;  // sequences with min_rows < query rows x group <= max_rows are taken, the others left alone
     float scale_log2e;       // scale * log2(e): scores are in log2 units
     int causal;
     bool bf16;
     bool to_state;           // write `out` instead of o
-    AttnState out;           // pieces = 1
+    AttnState out;           // where it goes, one piece for each split of the keys
     AttnState add;           // joined with the result before it is written; pieces = 0: none
-    float* part;             // split units' partial results
+    float* part;             // split units' partial results (kv_attention.cu)
 };
 
+// Few rows (kv_attention.cu). to_state writes one piece.
 size_t kv_attn_part_bytes();
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st);
+
+// Many rows (kv_attention_tc.cu): the keys of a unit are cut into `splits` pieces; more than one need to_state. Blocks of
+// 128 rows that a batch can have at most; the join of out's and add's pieces into o.
+int64_t kv_attn_tc_units(int64_t M, int batch, int group);
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, int splits, cudaStream_t st);
+cudaError_t launch_kv_state_join(const KvAttnArgs& a, cudaStream_t st);
 
 }  // namespace b2s
