@@ -79,18 +79,20 @@ int cache_view(const b2s_kv_cache* c, b2s::KvView* v, const char* op) {
 // kernel, which reads them once per 128.
 constexpr int kFewRows = 64;
 struct Plan {
-    bool few, many;
+    bool few, many, pair;
     int min_rows, splits;
 };
-Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys) {
-    Plan p{true, false, 0, 1};
+Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
+    Plan p{true, false, false, 0, 1};
     if (max_q * group <= kFewRows) return p;
     p.many = true;
     p.few = M != batch * max_q;  // equal: every sequence has max_q rows
     p.min_rows = p.few ? kFewRows : 0;
-    // Less than a wave of 128-row blocks: cut the keys, so that waves x (tiles of 128 keys + about four tiles' worth of
+    // Less than a wave of blocks: cut the keys, so that waves x (tiles of 128 keys + about four tiles' worth of
     // starting and ending a block) is least.
-    const int64_t units = std::max<int64_t>(1, M * group / 128) * kv_heads, tiles = (keys + 127) / 128;
+    p.pair = bf16 && max_q * group > 128;
+    const int block = p.pair ? 256 : 128;
+    const int64_t units = std::max<int64_t>(1, M * group / block) * kv_heads, tiles = (keys + 127) / 128;
     int64_t best = 0;
     for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles) && units < 148; ++s) {
         const int64_t cost = (units * s + 147) / 148 * ((tiles + s - 1) / s + 4) + (s > 1 ? 3 : 0);
@@ -162,8 +164,9 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     }
     if (prefix_len > 0 && !prefix_pages) return fail(B2S_ERR_INVALID_ARG, "%s: prefix_pages is NULL", op);
     const int group = n_heads / v.kv_heads;
-    const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift);
-    const Plan pre = plan_rows(M, 1, M, group, v.kv_heads, prefix_len);
+    const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift,
+                               type == B2S_TYPE_BF16);
+    const Plan pre = plan_rows(M, 1, M, group, v.kv_heads, prefix_len, type == B2S_TYPE_BF16);
     const AttnWs w = attn_ws(own, pre, M, n_heads, v.hd, prefix_len);
     if (!workspace || workspace_bytes < w.total)
         return fail(B2S_ERR_WORKSPACE, "%s needs %zu workspace bytes, got %zu", op, w.total, workspace ? workspace_bytes : 0);
@@ -182,6 +185,8 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     a.M = M;
     a.heads = n_heads;
     a.group = group;
+    while ((1u << a.group_shift) < (uint32_t)group) ++a.group_shift;  // n / group as a multiplication, for n < 2^31
+    a.group_mul = (uint32_t)((((uint64_t)1 << 32) * ((1u << a.group_shift) - (uint32_t)group)) / (uint32_t)group + 1);
     a.scale_log2e = scale * 1.4426950408889634f;
     a.bf16 = type == B2S_TYPE_BF16;
     a.part = reinterpret_cast<float*>(ws + w.part);
@@ -200,7 +205,7 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
         p.max_rows = (int)kMaxInt;
         p.to_state = true;
         p.out = state(w.prefix);
-        rc = launched(pre.many ? b2s::launch_kv_attention_tc(p, pre.splits, st) : b2s::launch_kv_attention(p, st), op);
+        rc = launched(pre.many ? b2s::launch_kv_attention_tc(p, pre.pair, pre.splits, st) : b2s::launch_kv_attention(p, st), op);
         if (rc) return rc;
         a.add = p.out;
     }
@@ -216,7 +221,7 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
         t.min_rows = own.min_rows;
         t.out = state(w.own);
         t.to_state = w.own.pieces > 0;
-        if ((rc = launched(b2s::launch_kv_attention_tc(t, own.splits, st), op))) return rc;
+        if ((rc = launched(b2s::launch_kv_attention_tc(t, own.pair, own.splits, st), op))) return rc;
         if (t.to_state && (rc = launched(b2s::launch_kv_state_join(t, st), op))) return rc;
     }
     if (!own.few) return B2S_OK;
@@ -308,9 +313,12 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache* cache, const b2s_kv_b
     if (cache_view(cache, &v, "attention_kv_workspace_size")) return 0;
     if (check_shapes(v, batch, M, n_heads, prefix_len, "attention_kv_workspace_size")) return 0;
     const int group = n_heads / v.kv_heads;
-    return attn_ws(plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift),
-                   plan_rows(M, 1, M, group, v.kv_heads, prefix_len), M, n_heads, v.hd, prefix_len)
-        .total;
+    size_t most = 0;
+    for (int bf16 = 0; bf16 < 2; ++bf16)  // either type
+        most = std::max(most, attn_ws(plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift, bf16),
+                                      plan_rows(M, 1, M, group, v.kv_heads, prefix_len, bf16), M, n_heads, v.hd, prefix_len)
+                                  .total);
+    return most;
 }
 
 int b2s_attention_kv(const b2s_kv_cache* cache, const b2s_kv_batch* batch, int32_t type, const void* q, int64_t ldq,

@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
 #pragma unroll
             for (int i = 0; i < HD / 4; ++i) x[i] = 0.0f;
             if (g < rows) {
-                const int r = row0 + g, i = r / a.group, head = h * a.group + (r - i * a.group);
+                const int r = row0 + g, i = a.by_group(r), head = h * a.group + (r - i * a.group);
                 limit = a.causal ? cw.s.len - cw.s.n + i + 1 : cw.s.len;
                 const int64_t at = (cw.s.lo + (int64_t)i) * a.ldq + (int64_t)head * a.c.hd + t * (HD / 4);
 #pragma unroll
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
             }
             if (cw.t0 == 0 && cw.t1 == cw.s.tiles) {
                 if (row < rows && d < a.c.hd) {
-                    const int r = row0 + row, i = r / a.group;
+                    const int r = row0 + row, i = a.by_group(r);
                     finish<N>(a, cw.s.lo + (int64_t)i, h * a.group + (r - i * a.group), d, mm, ll, o);
                 }
             } else {  // the first segment goes to slot 0, the last one to slot 1: no other can be cut
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(const KvAtt
         }
     }
     if (row < min(kRows, s.n * a.group - row0) && d < a.c.hd) {
-        const int r = row0 + row, i = r / a.group;
+        const int r = row0 + row, i = a.by_group(r);
         finish<N>(a, s.lo + (int64_t)i, h * a.group + (r - i * a.group), d, m, l, o);
     }
 }

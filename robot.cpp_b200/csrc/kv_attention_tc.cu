@@ -1,17 +1,23 @@
 // kv_attention_tc.cu -- attention of many query rows for each key/value head over the paged 8-bit cache, on the tcgen05
 // tensor cores: prompts, chunks of long prompts, and a batch's rows on a shared prefix.
 //
-// Mathematics as in kv_attention.cu: the 8-bit codes are exact in fp16, a query row scaled by a power of two is one
+// Mathematics as in kv_attention.cu: the 8-bit codes are exact in fp16; query rows scaled by a power of two are one
 // (bf16) or two (fp32) fp16 parts, and so are the probabilities times the value scale. One MMA a part:
 //   S = sum over parts Q_part K^T,  O += sum over parts P_part V   (fp32 accumulation in tensor memory).
-// Floor: 4 * pairs * hd operations a head times the parts, at the fp16 rate.
+// Floor: 4 * pairs * hd operations a head times the parts, at the fp16 rate; next to it the exponentials, 16 a clock and SM.
 //
-// A block holds 128 query rows (tokens x the heads of a group) of one sequence and key/value head and walks its keys in
-// tiles of 128. Warps 8-11 bring codes from the pages to registers, unpack them and store fp16 tiles in the 128-byte
-// swizzled layout that serves K as a K-major and V as an MN-major operand; warp 12 issues the MMAs; warps 0-7 hold two
-// threads for each row (64 keys each) and do the softmax from tensor memory, writing P over S. Three S/P buffers: the
-// scores of the next tile are computed while the softmax of this one runs.
-// The running maximum is moved only when a tile exceeds it by 2^8, so the outputs in tensor memory are rarely rescaled.
+// A block takes rows (tokens x the heads of a group) of one sequence and key/value head and walks its keys in tiles of 128.
+// Four warps bring codes from the pages, unpack them and store fp16 tiles in the 128-byte swizzled layout that serves K as a
+// K-major and V as an MN-major operand. Two groups of eight warps do the softmax from tensor memory, two threads a row, and
+// write P over S; one thread of each issues the group's MMAs. While one group's products run the other is at its
+// exponentials. Sixteen warps because one warp a scheduler needs 570 clocks for 32 keys' exponentials, four need 280 each
+// (measured alone; the special-function unit's own limit is 256). The groups are
+//   PAIR: two blocks of 128 rows that share every unpacked tile (bf16, where unpacking would weigh as much as the products);
+//   else: the even and the odd key tiles of the same 128 rows, each with its own reference, sum and outputs, joined at the
+//         end (fp32, whose two-part queries leave no room for more rows; and bf16 calls that have no more).
+// The reference of the exponentials is a whole number that moves only when probabilities grow past 2^8: sums, outputs and
+// the tile's probabilities are then multiplied by a power of two, which is exact. So scores are read once and no maximum is
+// formed: 32 probabilities whose sum is at most 2^8 are each at most that, and only a larger sum asks for their maximum.
 //
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
 // MMAs are issued, those in flight are waited for, and tensor memory is freed.
@@ -26,23 +32,27 @@ namespace b2s {
 
 namespace kvt {
 constexpr int kRows = 128, kKeys = 128;
-constexpr int kSoftWarps = 8, kConvWarps = 4, kThreads = 32 * (kSoftWarps + kConvWarps + 1);
-constexpr int kTmemCols = 512, kOcol = 384;  // S/P buffers at 0, 128, 256
+constexpr int kSoftWarps = 16, kConvWarps = 4, kThreads = 32 * (kSoftWarps + kConvWarps);
+constexpr int kTmemCols = 512, kOcol = 256;  // S/P of the two warpgroups at 0 and 128, O at 256 and 384
 constexpr int kBlock = kKeys * 128;          // bytes of 128 rows x 64 fp16 values
 struct Misc {
-    float ks[4][kKeys], vs[4][kKeys];  // scales of four tiles in flight
-    int vexp[4][kConvWarps];           // largest value-scale exponent of each 32 keys
-    uint32_t there[4][kConvWarps];     // keys that exist
-    float red[2][2][2][kRows];         // [tile parity][maximum, largest value scale][half][row]
-    float rf[kRows];                   // takes a row's scores back to log2 units
-    uint64_t kfull[2], kfree[2], vfull[2], vfree[2], sfull[3], pfull[3], pvd[3], scfull[4], drain;
-    int64_t scan[kSoftWarps + kConvWarps + 1];
+    float ks[4][kKeys];        // key scales of four tiles in flight, times the factor that takes scores to log2 units
+    float vs[4][kKeys];        // value scales
+    float vn[4][kKeys];        // value scales over the power of two above the largest finite one of their 32 keys
+    int vexp[4][kConvWarps];   // that one's biased exponent, 1..252
+    uint32_t there[4][kConvWarps];  // keys that exist
+    float m[2][2][kRows], l[2][2][kRows], back[2][kRows];  // [group][half of the row's keys][row]
+    int wmin[2][4];  // fewest keys that a row of a group's four row warps sees
+    uint64_t qfull, kfull[2], kfree[2], vfull[2], vfree[2], sfull[2], pvd[2], scfull[4], turn, drain[2];
+    int64_t scan[kThreads / 32];
     int64_t found[2];
+    float big[kSoftWarps];
     uint32_t tmem;
     int abort;
 };
-template <int HDP, int PARTS>
-constexpr size_t kSmem = 1024 + (size_t)(HDP / 64) * kBlock * (PARTS + 4) + sizeof(Misc);
+template <int HDP, int PARTS, bool PAIR>
+constexpr size_t kSmem = 1024 + (size_t)(HDP / 64) * kBlock * (PARTS * (PAIR ? 2 : 1) + 4) + kKeys * HDP + sizeof(Misc);
+static_assert(kSmem<128, 2, false> <= 232448 && kSmem<128, 1, true> <= 232448, "shared memory");
 }  // namespace kvt
 
 namespace {
@@ -69,16 +79,23 @@ __device__ __forceinline__ uint32_t pack_h2(float x0, float x1) {
     const __half2 h = __floats2half2_rn(x0, x1);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Four consecutive codes as two pairs of fp16. int8: 0x6400 | (b ^ 0x80) is 1152 + b; both steps are exact.
+// Four consecutive codes as two pairs of fp16: e4m3 (0, 1) and (2, 3), int8 (0, 2) and (1, 3), which saves it a byte
+// permutation; queries are stored in that order too, and outputs are taken out of it. int8: 0x6400 | (b ^ 0x80) is 1152 + b;
+// both steps are exact.
 template <bool E4M3>
 __device__ __forceinline__ void unpack4(uint32_t w, uint32_t& p0, uint32_t& p1) {
     if (E4M3) {
         p0 = e4m3x2_to_h2(w);
         p1 = e4m3x2_to_h2(w >> 16);
     } else {
-        p0 = sub_h2((__byte_perm(w, 0, 0x4140) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
-        p1 = sub_h2((__byte_perm(w, 0, 0x4342) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+        p0 = sub_h2((w & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
+        p1 = sub_h2(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0x64806480u);
     }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+    const int n = on ? 16 : 0;  // 0 bytes: nothing is read, zeros are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
 // V as an MN-major operand with 128-byte swizzle: 64 values of hd are 128 bytes, 8 keys make an atom (stride 1024), the
@@ -91,18 +108,27 @@ __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr) {
 constexpr uint32_t idesc_f16(int N, bool b_mn) {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 }
+// The MMAs and their commits are issued by one elected lane of a warp whose lanes all get here with the same operands: those
+// then live in uniform registers. (Under a branch on the lane every operand is moved there one by one: 150 clocks an MMA
+// where the tensor core needs 64.)
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -113,6 +139,31 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
         : "memory");
 }
 
+// Loads from tensor memory are complete behind this; the operands keep their uses behind it.
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28])
+                 :
+                 : "memory");
+    asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 // Paired fp32 operations (each lane an IEEE operation).
 struct F2 {
     uint64_t v;
@@ -121,6 +172,16 @@ __device__ __forceinline__ F2 f2(float a, float b) {
     F2 r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
     return r;
+}
+__device__ __forceinline__ F2 f2u(uint32_t a, uint32_t b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ void unf2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
@@ -140,7 +201,7 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
 }
 
 struct Rows {
-    int lo, n, len, tiles;  // first query row, query rows, keys, blocks of 128 (token, head of group) rows
+    int lo, n, len, rows;  // first query row, query rows, keys, (token, head of group) rows that this pass takes
 };
 __device__ __forceinline__ Rows rows_of(const KvAttnArgs& a, int b) {
     Rows s;
@@ -156,34 +217,45 @@ __device__ __forceinline__ Rows rows_of(const KvAttnArgs& a, int b) {
     }
     if (bad) atomicOr(&g_device_error, kErrIndex);
     s.len = (int)len;
-    s.tiles = s.n * a.group > a.min_rows ? (s.n * a.group + kRows - 1) / kRows : 0;
+    s.rows = s.n * a.group > a.min_rows ? s.n * a.group : 0;
     return s;
 }
 
-// A wait that ends: at its phase, after kWaitLimitNs, or at once when another wait of the block ran out.
-__device__ __forceinline__ bool wait(Misc* ms, uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
-    volatile int* ab = &ms->abort;
+// A wait that ends: at its phase, after kWaitLimitNs, or at once when another wait of the block ran out. The thread is
+// suspended for up to the hinted time at each try.
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(100000)
+        : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ void wait_on(int* abort, uint64_t* bar, uint32_t parity) {
+    volatile int* ab = abort;
     const uint64_t t0 = global_timer_ns();
-    for (uint32_t i = 0;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*ab) return false;
-        if ((i & 15u) == 15u && global_timer_ns() - t0 > kWaitLimitNs) break;
-    }
+    do {
+        if (*ab || try_wait(bar, parity)) return;
+    } while (global_timer_ns() - t0 <= kWaitLimitNs);
     *ab = 1;
     atomicOr(&g_device_error, 1u);
-    return false;
+}
+__device__ __forceinline__ void wait(Misc* ms, uint64_t* bar, uint32_t parity) {
+    if (!try_wait(bar, parity)) wait_on(&ms->abort, bar, parity);
 }
 
-template <int HDP, bool E4M3, int PARTS>
+template <int HDP, bool E4M3, int PARTS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAttnArgs a, int units, int splits) {
     constexpr int kTileBytes = HDP / 64 * kBlock;
+    constexpr int kBlkRows = PAIR ? 2 * kRows : kRows;  // rows of a block
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sK = sQ + PARTS * kTileBytes;
+    uint8_t* sK = sQ + PARTS * (PAIR ? 2 : 1) * kTileBytes;
     uint8_t* sV = sK + 2 * kTileBytes;
-    Misc* ms = reinterpret_cast<Misc*>(sV + 2 * kTileBytes);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* raw = sV + 2 * kTileBytes;  // the next value tile's codes
+    Misc* ms = reinterpret_cast<Misc*>(raw + kKeys * HDP);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // warp: the same in every lane
     griddep_wait();
     griddep_launch();
 
@@ -193,121 +265,93 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
     const int split = (int)(rest / units);
     int unit = (int)(rest - (int64_t)split * units);
     {
-        int64_t total = 0, w = 0, incl = 0;
-        for (int pass = 0; pass < 2; ++pass) {  // the total first: the order is from the last row block
-            int64_t before = 0;
-            for (int base = 0; base < a.batch; base += kThreads) {
-                const int b = base + tid;
-                w = b < a.batch ? rows_of(a, b).tiles : 0;
-                int64_t v = w;
+        auto scan = [&](int base, int64_t& w, int64_t& sum) {  // blocks of the sequences up to this thread's, and of all
+            const int b = base + tid;
+            w = b < a.batch ? (rows_of(a, b).rows + kBlkRows - 1) / kBlkRows : 0;
+            int64_t v = w;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-                    if (lane >= o) v += u;
-                }
-                __syncthreads();
-                if (lane == 31) ms->scan[warp] = v;
-                __syncthreads();
-                int64_t sum = 0;
-                for (int i = 0; i < kThreads / 32; ++i) {
-                    if (i < warp) v += ms->scan[i];
-                    sum += ms->scan[i];
-                }
-                incl = v + before;
-                before += sum;
-                if (pass == 1 && unit >= incl - w && unit < incl) {
-                    ms->found[0] = b;
-                    ms->found[1] = unit - (incl - w);
-                }
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
             }
-            if (pass == 0) {
-                total = before;
-                if (unit >= total) return;  // the grid is sized by a bound
-                unit = (int)(total - 1 - unit);
+            __syncthreads();
+            if (lane == 31) ms->scan[warp] = v;
+            __syncthreads();
+            sum = 0;
+            for (int i = 0; i < kThreads / 32; ++i) {
+                if (i < warp) v += ms->scan[i];
+                sum += ms->scan[i];
             }
+            return v;
+        };
+        int64_t total = 0, w = 0, sum = 0, incl = 0;
+        for (int base = 0; base < a.batch; base += kThreads) {
+            incl = scan(base, w, sum);
+            total += sum;
         }
-        __syncthreads();
+        if (unit >= total) return;  // the grid is sized by a bound
+        unit = (int)(total - 1 - unit);
+        int64_t before = total - sum;
+        for (int base = (a.batch - 1) / kThreads * kThreads;; base -= kThreads) {  // the last step's sums are at hand
+            incl += before;
+            if (unit >= incl - w && unit < incl) {
+                ms->found[0] = base + tid;
+                ms->found[1] = unit - (incl - w);
+            }
+            if (base == 0 || unit >= before) break;
+            incl = scan(base - kThreads, w, sum);
+            before -= sum;
+        }
     }
-    const int b = (int)ms->found[0], row0 = (int)ms->found[1] * kRows;
-    const Rows sq = rows_of(a, b);
-    const int rows = min(kRows, sq.n * a.group - row0);
-    // keys that the last row sees
-    const int most = a.causal ? min(sq.len, max(0, sq.len - sq.n + (row0 + rows - 1) / a.group + 1)) : sq.len;
-    const int all_tiles = (most + kKeys - 1) / kKeys;
-    const int t0 = (int)((int64_t)all_tiles * split / splits), nt = (int)((int64_t)all_tiles * (split + 1) / splits) - t0;
-
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ms->kfull[i], 32 * kConvWarps);
             mbar_init(&ms->vfull[i], 32 * kConvWarps);
-            mbar_init(&ms->kfree[i], 1);
-            mbar_init(&ms->vfree[i], 1);
-        }
-        for (int i = 0; i < 3; ++i) {
+            mbar_init(&ms->kfree[i], PAIR ? 2 : 1);
+            mbar_init(&ms->vfree[i], PAIR ? 2 : 1);
             mbar_init(&ms->sfull[i], 1);
-            mbar_init(&ms->pfull[i], 32 * kSoftWarps);
             mbar_init(&ms->pvd[i], 1);
+            mbar_init(&ms->drain[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&ms->scfull[i], 32 * kConvWarps);
-        mbar_init(&ms->drain, 1);
+        mbar_init(&ms->qfull, 32 * kSoftWarps);
+        mbar_init(&ms->turn, 2 * kRows);
         ms->abort = 0;
         fence_mbar_init();
     }
-    if (warp == kSoftWarps + kConvWarps) {
+    if (warp == kSoftWarps) {
         tmem_alloc(&ms->tmem, kTmemCols);
         tmem_relinquish();
-    }
-    // ---- the query rows: a warp takes a row at a time, four values a lane
-    const bool negative = a.scale_log2e < 0.0f, zero = a.scale_log2e == 0.0f;
-    if (warp < kSoftWarps) {
-        const int d = 4 * lane;
-#pragma unroll 4
-        for (int r = warp; r < kRows; r += kSoftWarps) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows && d < a.c.hd && !zero) {
-                const int i = (row0 + r) / a.group, head = h * a.group + (row0 + r - i * a.group);
-                const int64_t at = (sq.lo + (int64_t)i) * a.ldq + (int64_t)head * a.c.hd + d;
-                if (a.bf16) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + at);
-                    x = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                                    __uint_as_float(u.y & 0xffff0000u));
-                } else {
-                    x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at);
-                }
-            }
-            float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-            big = warp_max(big);
-            const int up = min(253, 268 - (__float_as_int(big) >> 23));  // the largest element goes to [2^14, 2^15)
-            const float mul = negative ? -pow2_biased(up) : pow2_biased(up);
-            if (lane == 0) ms->rf[r] = zero ? 1.0f : fmaxf(__fmul_rn(pow2_biased(254 - up), fabsf(a.scale_log2e)), 0x1p-126f);
-            const float y[4] = {__fmul_rn(x.x, mul), __fmul_rn(x.y, mul), __fmul_rn(x.z, mul), __fmul_rn(x.w, mul)};
-            if (d < HDP) {
-                uint8_t* p = sQ + (d >> 6) * kBlock + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2;
-                const uint2 hi = make_uint2(pack_h2(y[0], y[1]), pack_h2(y[2], y[3]));
-                *reinterpret_cast<uint2*>(p) = hi;
-                if (PARTS == 2) {
-                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
-                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-                    *reinterpret_cast<uint2*>(p + kTileBytes) = make_uint2(
-                        pack_h2(__fsub_rn(y[0], f0.x), __fsub_rn(y[1], f0.y)), pack_h2(__fsub_rn(y[2], f1.x), __fsub_rn(y[3], f1.y)));
-                }
-            }
-        }
-        fence_proxy_async_smem();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ms->tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, ms->tmem, 0);
+    const int b = (int)ms->found[0], row0 = (int)ms->found[1] * kBlkRows;
+    const Rows sq = rows_of(a, b);
+    const int rows = min(kBlkRows, sq.rows - row0);
+    // keys that the last row sees
+    const int most = a.causal ? min(sq.len, max(0, sq.len - sq.n + a.by_group(row0 + rows - 1) + 1)) : sq.len;
+    const int all_tiles = (most + kKeys - 1) / kKeys;
+    const int t0 = (int)((int64_t)all_tiles * split / splits), nt = (int)((int64_t)all_tiles * (split + 1) / splits) - t0;
 
-    if (warp >= kSoftWarps && warp < kSoftWarps + kConvWarps) {
+    // The power of two that all query rows share: the largest finite element goes to [2^14, 2^15).
+    auto common_up = [&]() {
+        float big = ms->big[0];
+#pragma unroll
+        for (int i = 1; i < kSoftWarps; ++i) big = fmaxf(big, ms->big[i]);
+        return min(253, 268 - (__float_as_int(big) >> 23));
+    };
+
+    if (warp >= kSoftWarps) {
         // ================================================================ codes to fp16 tiles
-        constexpr int kChunks = HDP / 16, kPer = kChunks;  // 16-byte code chunks of a row; chunks of a thread per tile
-        constexpr int kRowsPer = 32 / kChunks;             // rows that a warp covers at once
-        const int cw = warp - kSoftWarps, c = lane % kChunks, rsub = lane / kChunks;
+        // A warp has 32 keys of each tile. Four lanes take 64 codes of a key (one swizzled row of 128 bytes), eight keys at a
+        // time; chunk i is keys 8 (i / kBlk) + lane / 4 of block i % kBlk. Stores are free of bank conflicts.
+        constexpr int kBlk = HDP / 64, kChunks = 4 * kBlk;
+        float rf = 0.0f;  // takes scores back to log2 units
+        const int cw = warp - kSoftWarps, cc = lane & 3, rsub = lane >> 2;
         const int mask = (1 << a.c.page_shift) - 1;
         const int32_t* pg = a.pages + (int64_t)b * a.ld_pages;
-        const bool on_c = c * 16 < a.c.hd;
         // a warp's 32 keys of a tile lie in at most two pages: those of its first and its 17th key
         int pa = 0, pb = 0;
         auto fetch = [&](int j) {
@@ -315,331 +359,588 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             pa = k0 < sq.len ? pg[k0 >> a.c.page_shift] : 0;
             pb = k0 + 16 < sq.len ? pg[(k0 + 16) >> a.c.page_shift] : 0;
         };
-        int64_t ra = 0, rb = 0;
-        int k0 = 0;
-        bool ok_a = false, ok_b = false;
-        auto place = [&](int j) {
-            k0 = (t0 + j) * kKeys + cw * 32;
-            ok_a = pa >= 0 && pa < a.c.n_pages;
-            ok_b = pb >= 0 && pb < a.c.n_pages;
-            if (!(ok_a && ok_b) && lane == 0) atomicOr(&g_device_error, kErrIndex);
-            ra = (((int64_t)pa * a.c.kv_heads + h) << a.c.page_shift) + (k0 & mask);
-            rb = (((int64_t)pb * a.c.kv_heads + h) << a.c.page_shift) + ((k0 + 16) & mask) - 16;
+        struct Where {  // this lane's chunk in its first row of the first 16 keys, and of the others less 16 rows; keys there
+            int64_t ra, rb;
+            uint32_t bits;
         };
-        uint4 kr[kPer], vr[kPer];
-        float ksc = 0.0f, vsc = 0.0f;
-        bool here = false;
-        auto load = [&](const uint8_t* base, uint4 (&r)[kPer]) {
+        auto place = [&](int j) {
+            const int k0 = (t0 + j) * kKeys + cw * 32;
+            const bool ok_a = pa >= 0 && pa < a.c.n_pages, ok_b = pb >= 0 && pb < a.c.n_pages;
+            if (!(ok_a && ok_b) && lane == 0) atomicOr(&g_device_error, kErrIndex);
+            Where w;
+            w.ra = (((int64_t)pa * a.c.kv_heads + h) << a.c.page_shift) + (k0 & mask);
+            w.rb = (((int64_t)pb * a.c.kv_heads + h) << a.c.page_shift) + ((k0 + 16) & mask) - 16;
+            const int left = sq.len - k0;
+            w.bits = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+            if (!ok_a) w.bits &= 0xffff0000u;
+            if (!ok_b) w.bits &= 0x0000ffffu;
+            return w;
+        };
+        // The next key tile's codes wait in registers, the next value tile's in shared memory, where a thread copies the
+        // chunks that it unpacks itself.
+        uint4 kr[kChunks];
+        uint8_t* mine = raw + (tid - 32 * kSoftWarps) * 16;
+        auto load_values = [&](const Where& w) {
+            const uint8_t* p[2] = {a.c.v + (w.ra + rsub) * a.c.hd + cc * 16, a.c.v + (w.rb + rsub) * a.c.hd + cc * 16};
+            const uint32_t bits = w.bits >> rsub;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int row = i * kRowsPer + rsub;
+            for (int i = 0; i < kChunks; ++i) {
+                const int k = 8 * (i / kBlk);
+                const bool on = ((bits >> k) & 1) && (i % kBlk) * 64 + cc * 16 < a.c.hd;
+                cp_async16(smem_u32(mine) + i * (32 * kConvWarps * 16), on ? p[k / 16] + k * a.c.hd + (i % kBlk) * 64 : a.c.v, on);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        auto load = [&](const uint8_t* base, const Where& w, uint4 (&r)[kChunks]) {
+            const uint8_t* p[2] = {base + (w.ra + rsub) * a.c.hd + cc * 16, base + (w.rb + rsub) * a.c.hd + cc * 16};
+            const uint32_t bits = w.bits >> rsub;
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+                const int k = 8 * (i / kBlk);
                 r[i] = make_uint4(0, 0, 0, 0);
-                if ((row < 16 ? ok_a : ok_b) && k0 + row < sq.len && on_c)
-                    r[i] = __ldg(reinterpret_cast<const uint4*>(base + ((row < 16 ? ra : rb) + row) * a.c.hd + c * 16));
+                if (((bits >> k) & 1) && (i % kBlk) * 64 + cc * 16 < a.c.hd)
+                    r[i] = __ldg(reinterpret_cast<const uint4*>(p[k / 16] + k * a.c.hd + (i % kBlk) * 64));
             }
         };
-        auto load_scales = [&]() {
-            here = (lane < 16 ? ok_a : ok_b) && k0 + lane < sq.len;
+        float ksc = 0.0f, vsc = 0.0f;
+        auto load_scales = [&](const Where& w) {
             ksc = vsc = 0.0f;
-            if (here) {
-                const int64_t row = (lane < 16 ? ra : rb) + lane;
+            if ((w.bits >> lane) & 1) {
+                const int64_t row = (lane < 16 ? w.ra : w.rb) + lane;
                 ksc = __ldg(a.c.ks + row);
                 vsc = __ldg(a.c.vs + row);
             }
         };
-        auto store = [&](uint8_t* tile, const uint4 (&r)[kPer]) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int row = cw * 32 + i * kRowsPer + rsub;
-                uint32_t w[8];
-                unpack4<E4M3>(r[i].x, w[0], w[1]);
-                unpack4<E4M3>(r[i].y, w[2], w[3]);
-                unpack4<E4M3>(r[i].z, w[4], w[5]);
-                unpack4<E4M3>(r[i].w, w[6], w[7]);
-                uint8_t* p = tile + (c >> 2) * kBlock + row * 128;
-                const int ch = 2 * (c & 3), sw = (c >> 2) & 1;  // the second block's lanes store their halves in turn
-                const uint4 x0 = make_uint4(w[0], w[1], w[2], w[3]), x1 = make_uint4(w[4], w[5], w[6], w[7]);
-                *reinterpret_cast<uint4*>(p + (((ch + sw) ^ (row & 7)) << 4)) = sw ? x1 : x0;
-                *reinterpret_cast<uint4*>(p + (((ch + 1 - sw) ^ (row & 7)) << 4)) = sw ? x0 : x1;
-            }
+        const uint32_t at = (cw * 32 + rsub) * 128 + (((2 * cc) ^ rsub) << 4);
+        auto store = [&](uint8_t* tile, int i, uint4 r) {
+            uint32_t w[8];
+            unpack4<E4M3>(r.x, w[0], w[1]);
+            unpack4<E4M3>(r.y, w[2], w[3]);
+            unpack4<E4M3>(r.z, w[4], w[5]);
+            unpack4<E4M3>(r.w, w[6], w[7]);
+            const int off = (i % kBlk) * kBlock + (i / kBlk) * 1024;
+            *reinterpret_cast<uint4*>(tile + at + off) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(tile + (at ^ 16) + off) = make_uint4(w[4], w[5], w[6], w[7]);
         };
-        if (nt > 0) {
-            fetch(0);
-            place(0);
-            load(a.c.k, kr);
-            load_scales();
-            if (nt > 1) fetch(1);
-        }
-        for (int j = 0; j < nt; ++j) {
-            const int st = j & 1;
-            load(a.c.v, vr);  // this tile's places are still set
+        // Order of the tiles: K0, K1, V0, K2, V1, ...: the next tile's scores do not wait for this one's V. Each is asked for
+        // when the one before it of its kind has been stored.
+        Where pk{}, pv{};  // places of the keys and values asked for last
+        auto ask_keys = [&](int j) {
+            pv = pk;
+            if (j >= nt) return;
+            pk = place(j);
+            load(a.c.k, pk, kr);
+            load_scales(pk);
+            if (j + 1 < nt) fetch(j + 1);
+        };
+        auto keys = [&](int j) {
+            const int st = j & 1, sc = j & 3;
             if (j >= 2) wait(ms, &ms->kfree[st], (uint32_t)((j >> 1) - 1) & 1u);
-            store(sK + st * kTileBytes, kr);
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) store(sK + st * kTileBytes, i, kr[i]);
             fence_proxy_async_smem();
             mbar_arrive(&ms->kfull[st]);
-            ms->ks[j & 3][cw * 32 + lane] = ksc;
-            ms->vs[j & 3][cw * 32 + lane] = vsc;
-            const int e = __reduce_max_sync(0xffffffffu, here ? (__float_as_int(fabsf(vsc)) >> 23) : 0);
-            const uint32_t bits = __ballot_sync(0xffffffffu, here);
+            if (j == 0) {
+                wait(ms, &ms->qfull, 0);
+                rf = __fmul_rn(pow2_biased(254 - common_up()), a.scale_log2e);
+            }
+            ms->ks[sc][cw * 32 + lane] = __fmul_rn(ksc, rf);
+            ms->vs[sc][cw * 32 + lane] = vsc;
+            int e = __float_as_int(fabsf(vsc)) >> 23;
+            e = __reduce_max_sync(0xffffffffu, e == 255 ? 1 : max(1, min(252, e)));
+            ms->vn[sc][cw * 32 + lane] = __fmul_rn(vsc, pow2_biased(253 - e));
             if (lane == 0) {
-                ms->vexp[j & 3][cw] = e;
-                ms->there[j & 3][cw] = bits;
+                ms->vexp[sc][cw] = e;
+                ms->there[sc][cw] = pk.bits;
             }
             __syncwarp();
-            mbar_arrive(&ms->scfull[j & 3]);
-            if (j + 1 < nt) {
-                place(j + 1);
-                load(a.c.k, kr);
-                load_scales();
-                if (j + 2 < nt) fetch(j + 2);
+            mbar_arrive(&ms->scfull[sc]);
+        };
+        if (nt > 0) fetch(0);
+#pragma unroll 1
+        for (int j = -2; j < nt; ++j) {  // one copy of each step: the code of a turn has to stay in the instruction cache
+            const bool more = j >= -1 && j + 1 < nt;
+            if (more) keys(j + 1);
+            ask_keys(j + 2);
+            if (j >= 0) {
+                if (j >= 2) wait(ms, &ms->vfree[j & 1], (uint32_t)((j >> 1) - 1) & 1u);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 2
+                for (int i = 0; i < kChunks; ++i)
+                    store(sV + (j & 1) * kTileBytes, i, *reinterpret_cast<const uint4*>(mine + i * (32 * kConvWarps * 16)));
+                fence_proxy_async_smem();
+                mbar_arrive(&ms->vfull[j & 1]);
             }
-            if (j >= 2) wait(ms, &ms->vfree[st], (uint32_t)((j >> 1) - 1) & 1u);
-            store(sV + st * kTileBytes, vr);
-            fence_proxy_async_smem();
-            mbar_arrive(&ms->vfull[st]);
+            if (more) load_values(pv);
         }
-    } else if (warp == kSoftWarps + kConvWarps) {
-        // ================================================================ MMAs
-        if (lane == 0) {
-            constexpr uint32_t kIdS = idesc_f16(kKeys, false), kIdO = idesc_f16(HDP, true);
-            const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
-            bool ok = true;
-            auto scores = [&](int j) {
-                ok = wait(ms, &ms->kfull[j & 1], (uint32_t)(j >> 1) & 1u) && ok;
-                // the buffer's last reader, the product with the probabilities of tile j - 3, has to be through
-                if (j >= 3) ok = wait(ms, &ms->pvd[j % 3], (uint32_t)(j / 3 - 1) & 1u) && ok;
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(j % 3) * kKeys, kt = k0 + (j & 1) * kTileBytes;
-#pragma unroll
-                for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                    for (int s = 0; s < HDP / 16; ++s) {
-                        const uint32_t off = (s >> 2) * kBlock + (s & 3) * 32;
-                        mma_ss(d, umma_desc_k_sw128(q0 + part * kTileBytes + off), umma_desc_k_sw128(kt + off), kIdS,
-                               (part > 0 || s > 0) ? 1u : 0u);
-                    }
-                tc_commit(&ms->sfull[j % 3]);
-                tc_commit(&ms->kfree[j & 1]);
-            };
-            if (nt > 0) scores(0);
-            for (int j = 0; j < nt; ++j) {
-                if (j + 1 < nt) scores(j + 1);
-                ok = wait(ms, &ms->vfull[j & 1], (uint32_t)(j >> 1) & 1u) && ok;
-                ok = wait(ms, &ms->pfull[j % 3], (uint32_t)(j / 3) & 1u) && ok;
-                if (!ok) continue;
-                tc_fence_after();
-                const uint32_t p = tmem + (uint32_t)(j % 3) * kKeys, vt = v0 + (j & 1) * kTileBytes;
-#pragma unroll
-                for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                    for (int s = 0; s < kKeys / 16; ++s)
-                        mma_ts(tmem + kOcol, p + part * 64 + s * 8, desc_mn_sw128(vt + s * 2048), kIdO,
-                               (j > 0 || part > 0 || s > 0) ? 1u : 0u);
-                tc_commit(&ms->pvd[j % 3]);
-                tc_commit(&ms->vfree[j & 1]);
-            }
-            if (!ok) {  // let what was issued finish before tensor memory is freed
-                tc_commit(&ms->drain);
-                mbar_wait(&ms->drain, 0, 2u);
-            }
-        }
-        __syncwarp();
     } else {
         // ================================================================ softmax
-        const int quad = warp & 3, half = warp >> 2, r = quad * 32 + lane;
+        // ---- the query rows, 16 bytes a lane: two bf16 rows or one fp32 row for each warp and load
+        {
+            constexpr int kPer = PARTS == 2 ? 1 : 2, kQr = kBlkRows / kSoftWarps / kPer;
+            constexpr int kVals = PARTS == 2 ? 4 : 8, kLanes = 32 / kPer;
+            const int sub = lane / kLanes, d = (lane % kLanes) * kVals, dd = min(d, a.c.hd - kVals);
+            uint4 q[kQr];
+            const int first = warp * kPer + sub;  // rows first, first + 16 kPer, ...
+#pragma unroll
+            for (int k = 0; k < kQr; ++k) {  // all loads are in flight before the first is used; what is not there is dropped
+                const int rr = row0 + min(first + k * kSoftWarps * kPer, rows - 1), ti = a.by_group(rr);
+                const int64_t at = (sq.lo + (int64_t)ti) * a.ldq + (int64_t)(h * a.group + (rr - ti * a.group)) * a.c.hd + dd;
+                q[k] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + at * (PARTS == 2 ? 4 : 2));
+            }
+            auto values = [&](uint4 u, bool on, float (&x)[kVals]) {
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int i = 0; i < kVals; ++i) {
+                    const float y = PARTS == 2 ? __uint_as_float(w[i & 3])
+                                               : __uint_as_float((i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+                    x[i] = on ? y : 0.0f;
+                }
+            };
+            float big = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kQr; ++k) {
+                float x[kVals];
+                values(q[k], first + k * kSoftWarps * kPer < rows && d < a.c.hd, x);
+#pragma unroll
+                for (int i = 0; i < kVals; ++i) {
+                    const float y = fabsf(x[i]);
+                    big = fmaxf(big, y < INFINITY ? y : 0.0f);
+                }
+            }
+            big = warp_max(big);
+            if (lane == 0) ms->big[warp] = big;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            const float mul = pow2_biased(common_up());
+            if (d < HDP) {
+#pragma unroll
+                for (int k = 0; k < kQr; ++k) {
+                    const int r = first + k * kSoftWarps * kPer, rr = r & (kRows - 1);
+                    float x[kVals];
+                    values(q[k], r < rows && d < a.c.hd, x);
+                    uint32_t hi[kVals / 2];
+                    float y[kVals];
+#pragma unroll
+                    for (int i = 0; i < kVals; i += 4) {  // in the order of unpack4's pairs
+                        y[i] = __fmul_rn(x[i], mul);
+                        y[i + 1] = __fmul_rn(x[i + (E4M3 ? 1 : 2)], mul);
+                        y[i + 2] = __fmul_rn(x[i + (E4M3 ? 2 : 1)], mul);
+                        y[i + 3] = __fmul_rn(x[i + 3], mul);
+                        hi[i / 2] = pack_h2(y[i], y[i + 1]);
+                        hi[i / 2 + 1] = pack_h2(y[i + 2], y[i + 3]);
+                    }
+                    uint8_t* p = sQ + (PAIR ? (r >> 7) * kTileBytes : 0) + (d >> 6) * kBlock + rr * 128 +
+                                 ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 4) * 2;
+                    if constexpr (PARTS == 1) {
+                        *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    } else {
+                        *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[1]);
+                        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi[0]));
+                        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi[1]));
+                        *reinterpret_cast<uint2*>(p + kTileBytes) =
+                            make_uint2(pack_h2(__fsub_rn(y[0], f0.x), __fsub_rn(y[1], f0.y)),
+                                       pack_h2(__fsub_rn(y[2], f1.x), __fsub_rn(y[3], f1.y)));
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&ms->qfull);
+        }
+        const int wg = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-        const bool mine = r < rows;
-        const int tok = (row0 + r) / a.group;
+        const uint32_t sbuf = lane_addr + wg * kKeys, obuf = lane_addr + kOcol + wg * kRows + half * (HDP / 2);
+        const int rb = row0 + (PAIR ? wg * kRows : 0) + r;  // row of the sequence
+        const bool mine = rb < row0 + rows;
+        const int tok = a.by_group(rb);
         // a row that is not there never masks (its results are dropped)
         const int limit = !mine ? 0x7fffffff : a.causal ? sq.len - sq.n + tok + 1 : sq.len;
-        const int wmin = __reduce_min_sync(0xffffffffu, limit);
-        const float rf = ms->rf[r];
-        float m = -INFINITY, l = 0.0f;
-        int vref = 8;
-        for (int j = 0; j < nt; ++j) {
-            const int key0 = (t0 + j) * kKeys + half * 64;
-            wait(ms, &ms->scfull[j & 3], (uint32_t)(j >> 2) & 1u);
-            const uint32_t w0 = ms->there[j & 3][2 * half], w1 = ms->there[j & 3][2 * half + 1];
-            const uint32_t wo = ms->there[j & 3][2 - 2 * half] & ms->there[j & 3][3 - 2 * half];
-            const bool masked = (w0 & w1 & wo) != 0xffffffffu || (t0 + j + 1) * kKeys > wmin;
-            const float4* ksp = reinterpret_cast<const float4*>(&ms->ks[j & 3][half * 64]);
-            const float4* vsp = reinterpret_cast<const float4*>(&ms->vs[j & 3][half * 64]);
-            int e = max(max(ms->vexp[j & 3][0], ms->vexp[j & 3][1]), max(ms->vexp[j & 3][2], ms->vexp[j & 3][3]));
-            wait(ms, &ms->sfull[j % 3], (uint32_t)(j / 3) & 1u);
-            tc_fence_after();
-            const uint32_t sbuf = lane_addr + (uint32_t)(j % 3) * kKeys;
-            float s[64];
-            {
-                uint32_t x[32], y[32];
-                tmem_ld_32x32b_x32(sbuf + half * 64, x);
-                tmem_ld_32x32b_x32(sbuf + half * 64 + 32, y);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    s[i] = __uint_as_float(x[i]);
-                    s[32 + i] = __uint_as_float(y[i]);
-                }
-            }
-            float mx = -INFINITY, vmx = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float4 f = ksp[i];
-                unf2(mul2(f2(s[4 * i], s[4 * i + 1]), f2(f.x, f.y)), s[4 * i], s[4 * i + 1]);
-                unf2(mul2(f2(s[4 * i + 2], s[4 * i + 3]), f2(f.z, f.w)), s[4 * i + 2], s[4 * i + 3]);
-            }
-            uint32_t see0 = 0xffffffffu, see1 = 0xffffffffu;  // keys of this thread that the row sees
-            if (masked) {
-                const int left = limit - key0;
-                see0 = w0 & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
-                see1 = w1 & (left >= 64 ? 0xffffffffu : left > 32 ? (1u << (left - 32)) - 1u : 0u);
-                const float* vp = &ms->vs[j & 3][half * 64];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if (!((see0 >> i) & 1)) s[i] = -INFINITY; else vmx = fmaxf(vmx, fabsf(vp[i]));
-                    if (!((see1 >> i) & 1)) s[32 + i] = -INFINITY; else vmx = fmaxf(vmx, fabsf(vp[32 + i]));
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i]);
-            // ---- the row's two threads: from here on S is in registers, and P may be written over it
-            ms->red[j & 1][0][half][r] = mx;
-            if (masked) ms->red[j & 1][1][half][r] = vmx;
+        {
+            const int w = __reduce_min_sync(0xffffffffu, limit);
+            if (half == 0 && lane == 0) ms->wmin[wg][quad] = w;
+        }
+        auto group_sync = [&]() {
             tc_fence_before();
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+            asm volatile("bar.sync %0, 256;" ::"r"(2 + wg) : "memory");
             tc_fence_after();
-            mx = fmaxf(mx, ms->red[j & 1][0][half ^ 1][r]);
-            if (masked) e = __float_as_int(fmaxf(vmx, ms->red[j & 1][1][half ^ 1][r])) >> 23;
-            const float mt = __fmul_rn(mx, rf);
-            const bool move = mt > __fadd_rn(m, 8.0f) || (m == -INFINITY && mt > -INFINITY) || e >= vref;
-            if (__any_sync(0xffffffffu, move)) {
+        };
+        auto group_any = [&](bool x) {  // whether any thread of the group has x; a barrier
+            uint32_t y = x;
+            tc_fence_before();
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbar.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                : "+r"(y)
+                : "r"(2 + wg)
+                : "memory");
+            tc_fence_after();
+            return y != 0;
+        };
+        group_sync();
+        const int wmin = min(min(ms->wmin[wg][0], ms->wmin[wg][1]), min(ms->wmin[wg][2], ms->wmin[wg][3]));
+        const int n = PAIR ? nt : (nt + 1 - wg) / 2;
+        float m = -INFINITY, l = 0.0f;  // the two threads of a row have the same m, and l of their keys
+        int vref = 8;
+        // ---- this group's MMAs, issued by its first warp
+        const bool leader = (warp & 7) == 0;
+        const uint32_t q0 = smem_u32(sQ) + (PAIR ? wg * kTileBytes : 0), s0 = tmem + wg * kKeys, o0 = tmem + kOcol + wg * kRows;
+        volatile int* ab = &ms->abort;
+        auto issue_scores = [&](int i) {
+            const int j = PAIR ? i : 2 * i + wg;
+            wait(ms, &ms->kfull[j & 1], (uint32_t)(j >> 1) & 1u);
+            if (__any_sync(0xffffffffu, *ab)) return;
+            tc_fence_after();
+            const uint32_t kt = smem_u32(sK) + (j & 1) * kTileBytes;
+            const uint64_t qd = umma_desc_k_sw128(q0), kd = umma_desc_k_sw128(kt);
+#pragma unroll
+            for (int k = 0; k < PARTS * (HDP / 16); ++k) {  // the small part first: fewer roundings of large sums
+                const int part = PARTS - 1 - k / (HDP / 16), s = k % (HDP / 16);
+                const uint32_t off = ((s >> 2) * kBlock + (s & 3) * 32) >> 4;
+                mma_ss(s0, qd + (part * kTileBytes >> 4) + off, kd + off, idesc_f16(kKeys, false), k > 0 ? 1u : 0u);
+            }
+            commit_elected(&ms->sfull[wg]);
+            commit_elected(&ms->kfree[j & 1]);
+        };
+        auto issue_outputs = [&](int i) {
+            const int j = PAIR ? i : 2 * i + wg;
+            wait(ms, &ms->vfull[j & 1], (uint32_t)(j >> 1) & 1u);
+            if (__any_sync(0xffffffffu, *ab)) return;
+            tc_fence_after();
+            const uint32_t vt = smem_u32(sV) + (j & 1) * kTileBytes;
+            const uint64_t vd = desc_mn_sw128(vt);
+#pragma unroll
+            for (int k = 0; k < PARTS * (kKeys / 16); ++k) {  // P of 32 keys: 16 columns of the large parts, 16 of the small ones
+                const int part = PARTS - 1 - k / (kKeys / 16), s = k % (kKeys / 16);
+                mma_ts(o0, s0 + (s >> 1) * 32 + part * 16 + (s & 1) * 8, vd + (s * 2048 >> 4), idesc_f16(HDP, true),
+                       k > 0 ? 1u : i > 0 ? 1u : 0u);
+            }
+            commit_elected(&ms->pvd[wg]);
+            commit_elected(&ms->vfree[j & 1]);
+        };
+        if (leader) {
+            wait(ms, &ms->qfull, 0);
+            if (PAIR && wg == 1 && n > 0) wait(ms, &ms->turn, 0);  // half a tile behind: one computes while the other's products run
+        }
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const int j = PAIR ? i : 2 * i + wg, sc = j & 3;
+            if (leader) {
+                if (i > 0) wait(ms, &ms->pvd[wg], (uint32_t)(i - 1) & 1u);  // these scores overwrite P
+                issue_scores(i);
+            }
+            __syncwarp();
+            wait(ms, &ms->scfull[sc], (uint32_t)(j >> 2) & 1u);
+            const uint4 there = *reinterpret_cast<const uint4*>(ms->there[sc]);
+            const int key0 = (t0 + j) * kKeys;
+            const bool edge = (there.x & there.y & there.z & there.w) != 0xffffffffu || key0 + kKeys > wmin;
+            // keys of 32 that the row sees
+            auto see_of = [&](int c) {
+                const int left = limit - (key0 + 32 * c);
+                return ms->there[sc][c] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
+            };
+            wait(ms, &ms->sfull[wg], (uint32_t)i & 1u);
+            // Every choice between barriers is the group's, by a barrier of its own: it is one even if a wait ran out.
+            const bool masked = group_any(edge);
+            // From here on the outputs of the last tile are complete.
+            auto scale_outputs = [&](float f) {  // this thread's half of the columns
+                if (i == 0) return;
+#pragma unroll 1
+                for (int c = 0; c < HDP / 2; c += 16) {
+                    uint32_t x[16];
+                    tmem_ld_x16(obuf + c, x);
+                    wait_ld(x);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__fmul_rn(__uint_as_float(x[k]), f));
+                    tmem_st_x16(obuf + c, x);
+                }
+            };
+            auto scale_probabilities = [&](int c0, int c1, float f) {  // chunks c0 .. c1 - 1 of the tile
+                tc_wait_st();
+                const __half2 f2h = __float2half2_rn(f);
+#pragma unroll 1
+                for (int c = 32 * c0; c < 32 * c1; c += PARTS == 1 ? 32 : 16) {
+                    uint32_t x[16];
+                    tmem_ld_x16(sbuf + c, x);
+                    wait_ld(x);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&x[k]), f2h);
+                        x[k] = *reinterpret_cast<const uint32_t*>(&z);
+                    }
+                    tmem_st_x16(sbuf + c, x);
+                }
+            };
+            // 2^(from - to) for whole numbers from <= to; 0 from -inf
+            auto down = [&](float from, float to) {
+                const float by = __fsub_rn(from, to);
+                return by >= -126.0f ? pow2_biased(127 + (int)by) : 0.0f;
+            };
+            // The power of two that value scales are kept under; e is the same for a row's two threads.
+            auto widen = [&](int e) {
+                const bool up = e >= vref;
+                if (!__any_sync(0xffffffffu, up)) return;
                 float f = 1.0f;
-                if (move) {
-                    const float mn = fmaxf(m, mt);
-                    f = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, mn));
-                    l = __fmul_rn(l, f);
-                    m = mn;
-                    const int nref = e >= vref ? min(e + 2, 255) : vref;
-                    f = nref - vref > 126 ? 0.0f : __fmul_rn(f, pow2_biased(127 - (nref - vref)));
+                if (up) {
+                    const int nref = min(e + 2, 255);
+                    f = nref - vref > 126 ? 0.0f : pow2_biased(127 - (nref - vref));
                     vref = nref;
                 }
-                if (j > 0) {
-                    wait(ms, &ms->pvd[(j - 1) % 3], (uint32_t)((j - 1) / 3) & 1u);
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < HDP / 2; c += 16) {
-                        const uint32_t at = lane_addr + kOcol + half * (HDP / 2) + c;
-                        uint32_t x[16];
-                        tmem_ld_x16(at, x);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__fmul_rn(__uint_as_float(x[i]), f));
-                        tmem_st_x16(at, x);
-                    }
+                scale_outputs(f);
+            };
+            auto part = [&](F2 w, uint32_t& hi, uint32_t& lo) {
+                float u, v;
+                unf2(w, u, v);
+                hi = pack_h2(u, v);
+                if (PARTS == 2) {
+                    const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                    unf2(add2(w, f2(-b2.x, -b2.y)), u, v);
+                    lo = pack_h2(u, v);
                 }
-            }
-            const float mu = m == -INFINITY ? 0.0f : -m, vmul = pow2_biased(260 - vref);
-            const F2 rf2 = f2(rf, rf), mu2 = f2(mu, mu), vmul2 = f2(vmul, vmul);
-            F2 l2 = f2(0.0f, 0.0f);
+            };
+            if (!masked) {
+                const int4 ve = *reinterpret_cast<const int4*>(ms->vexp[sc]);
+                widen(max(max(ve.x, ve.y), max(ve.z, ve.w)));
+                // P of 32 keys over their scores: p = 2^(s - m + shift) times the value scales, which are over 2^(exponent + 1)
+                // of their 32 keys (one far below the reference counts as 2^-60); their sum is taken back by 2^-shift
+                const float m0 = m;
+#pragma unroll 1
+                for (int c = 2 * half; c < 2 * half + 2; ++c) {
+                    const float4* ksp = reinterpret_cast<const float4*>(&ms->ks[sc][32 * c]);
+                    const float4* vnp = reinterpret_cast<const float4*>(&ms->vn[sc][32 * c]);
+                    const int shift = max(-60, ms->vexp[sc][c] + 7 - vref);
+                    const float most = pow2_biased(127 + 8 + shift);
+                    uint32_t x[32];
+                    float sum;
+                    tmem_ld_32x32b_x32(sbuf + 32 * c, x);
+                    wait_ld(x);
+                    for (bool again = false;; again = true) {
+                        const float cc = __fsub_rn((float)shift, m);
+                        const F2 c2 = f2(cc, cc);
+                        F2 sum0 = f2(0.0f, 0.0f), sum1 = sum0;
+                        float u, v;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                uint32_t hi[16], lo[16];
+                        for (int q = 0; q < 2; ++q) {  // P of 16 keys at a time
+                            uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 f = vsp[q * 8 + i];
-                    float fv[4] = {f.x, f.y, f.z, f.w};
-                    if (masked) {  // a value scale that the row does not see may be anything
-                        const uint32_t see = (q ? see1 : see0) >> (4 * i);
+                            for (int k = 0; k < 4; ++k) {
+                                const float4 f = ksp[4 * q + k], g = vnp[4 * q + k];
+                                const uint32_t* xk = &x[16 * q + 4 * k];
+                                unf2(fma2(f2u(xk[0], xk[1]), f2(f.x, f.y), c2), u, v);
+                                F2 p = f2(ex2(u), ex2(v));
+                                sum0 = add2(sum0, p);
+                                part(mul2(p, f2(g.x, g.y)), hi[2 * k], lo[2 * k]);
+                                unf2(fma2(f2u(xk[2], xk[3]), f2(f.z, f.w), c2), u, v);
+                                p = f2(ex2(u), ex2(v));
+                                sum1 = add2(sum1, p);
+                                part(mul2(p, f2(g.z, g.w)), hi[2 * k + 1], lo[2 * k + 1]);
+                            }
+                            tmem_st_x8(sbuf + 32 * c + 8 * q, hi);
+                            if (PARTS == 2) tmem_st_x8(sbuf + 32 * c + 16 + 8 * q, lo);
+                        }
+                        unf2(add2(sum0, sum1), u, v);
+                        sum = __fadd_rn(u, v);
+                        // too large at first (m is -inf), where the scores have grown, and for NaN
+                        if (again || !__any_sync(0xffffffffu, !(sum <= most))) break;
+                        float mx = -INFINITY;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (!((see >> k) & 1)) fv[k] = 0.0f;
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 f = ksp[k];
+                            mx = max3(mx, __fmul_rn(__uint_as_float(x[4 * k]), f.x), __fmul_rn(__uint_as_float(x[4 * k + 1]), f.y));
+                            mx = max3(mx, __fmul_rn(__uint_as_float(x[4 * k + 2]), f.z), __fmul_rn(__uint_as_float(x[4 * k + 3]), f.w));
+                        }
+                        // m follows here for this thread's keys, and for the row behind the barrier
+                        float f = 1.0f;
+                        if (mx > __fadd_rn(m, 8.0f)) {
+                            const float mn = ceilf(mx);
+                            f = down(m, mn);
+                            l = __fmul_rn(l, f);
+                            m = mn;
+                        }
+                        if (c & 1) scale_probabilities(c - 1, c, f);
                     }
+                    l = __fmaf_rn(sum, pow2_biased(127 - shift), l);
+                }
+                ms->m[wg][half][r] = m;
+                tc_wait_st();
+                const bool moved = group_any(m != m0);
+                if (moved) {
+                    const float mn = fmaxf(m, ms->m[wg][half ^ 1][r]), f = down(m, mn);
+                    if (__any_sync(0xffffffffu, m != mn)) {
+                        scale_probabilities(2 * half, 2 * half + 2, f);
+                        l = __fmul_rn(l, f);
+                    }
+                    scale_outputs(down(m0, mn));
+                    m = mn;
+                    tc_wait_st();
+                    group_sync();
+                }
+            } else {  // a key or value scale that the row does not see may be anything
+                float mx = -INFINITY, vmx = 0.0f;
+#pragma unroll 1
+                for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                    const uint32_t see = see_of(c >> 1) >> (16 * (c & 1));
+                    uint32_t x[16];
+                    tmem_ld_x16(sbuf + 16 * c, x);
+                    wait_ld(x);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int at = q * 32 + 4 * i + 2 * k;
-                        float x0, x1;
-                        unf2(fma2(f2(s[at], s[at + 1]), rf2, mu2), x0, x1);
-                        const F2 p = f2(ex2(x0), ex2(x1));
-                        l2 = add2(l2, p);
-                        unf2(mul2(p, mul2(f2(fv[2 * k], fv[2 * k + 1]), vmul2)), x0, x1);
-                        hi[2 * i + k] = pack_h2(x0, x1);
-                        if (PARTS == 2) {
-                            const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&hi[2 * i + k]));
-                            lo[2 * i + k] = pack_h2(__fsub_rn(x0, b2.x), __fsub_rn(x1, b2.y));
+                    for (int k = 0; k < 16; ++k) {
+                        const float u = __fmul_rn(__uint_as_float(x[k]), ms->ks[sc][16 * c + k]);
+                        if ((see >> k) & 1) {
+                            mx = fmaxf(mx, u);
+                            vmx = fmaxf(vmx, fabsf(ms->vs[sc][16 * c + k]));
                         }
                     }
                 }
-                tmem_st_x16(sbuf + half * 32 + q * 16, hi);
-                if (PARTS == 2) tmem_st_x16(sbuf + 64 + half * 32 + q * 16, lo);
+                ms->m[wg][half][r] = mx;
+                ms->l[wg][half][r] = vmx;
+                group_sync();
+                mx = fmaxf(mx, ms->m[wg][half ^ 1][r]);
+                vmx = fmaxf(vmx, ms->l[wg][half ^ 1][r]);
+                widen(__float_as_int(vmx) >> 23);
+                const bool up = mx > __fadd_rn(m, 8.0f);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float mn = up ? ceilf(mx) : m, f = up ? down(m, mn) : 1.0f;
+                    l = __fmul_rn(l, f);
+                    m = mn;
+                    tc_wait_st();
+                    scale_outputs(f);
+                }
+                const float mu = m == -INFINITY ? 0.0f : -m, vmul = pow2_biased(260 - vref);
+                uint32_t keep[8];
+#pragma unroll 1
+                for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                    const uint32_t see = see_of(c >> 1) >> (16 * (c & 1));
+                    uint32_t x[16];
+                    tmem_ld_x16(sbuf + 16 * c, x);
+                    float sum = 0.0f;
+                    uint32_t hi[8], lo[8];
+                    wait_ld(x);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        float p[2], w[2];
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const int key = 16 * c + 2 * k + q;
+                            const bool on = (see >> (2 * k + q)) & 1;
+                            p[q] = on ? ex2(__fmaf_rn(__uint_as_float(x[2 * k + q]), ms->ks[sc][key], mu)) : 0.0f;
+                            w[q] = on ? __fmul_rn(p[q], __fmul_rn(ms->vs[sc][key], vmul)) : 0.0f;
+                        }
+                        sum = __fadd_rn(sum, __fadd_rn(p[0], p[1]));
+                        part(f2(w[0], w[1]), hi[k], lo[k]);
+                    }
+                    const uint32_t to = sbuf + 32 * (c >> 1) + 8 * (c & 1);
+                    // the chunk's second 16 scores lie where its small parts go: they are kept until those are read
+                    if (PARTS == 1) {
+                        tmem_st_x8(to, hi);
+                    } else if (c & 1) {
+                        tmem_st_x8(to, hi);
+                        tmem_st_x8(to + 16, lo);
+                        tmem_st_x8(to + 8, keep);
+                    } else {
+                        tmem_st_x8(to, hi);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) keep[k] = lo[k];
+                    }
+                    l = __fadd_rn(l, sum);
+                }
+                tc_wait_st();
+                group_sync();
             }
-            float la, lb;
-            unf2(l2, la, lb);
-            l = __fadd_rn(l, __fadd_rn(la, lb));
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&ms->pfull[j % 3]);
+            if (PAIR && wg == 0 && i == 0) mbar_arrive(&ms->turn);
+            if (leader) issue_outputs(i);
+            __syncwarp();
         }
-        // ---- the row's sum, and the outputs: each of its two threads writes half of the columns
-        ms->red[nt & 1][0][half][r] = l;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-        l = __fadd_rn(ms->red[nt & 1][0][0][r], ms->red[nt & 1][0][1][r]);
-        if (nt > 0) {
-            wait(ms, &ms->pvd[(nt - 1) % 3], (uint32_t)((nt - 1) / 3) & 1u);
+        if (n > 0) {
+            wait(ms, &ms->pvd[wg], (uint32_t)(n - 1) & 1u);
             tc_fence_after();
         }
-        const float back = pow2_biased(vref - 6);
+        if (leader) {  // also after a wait that ran out: what was issued finishes before tensor memory is freed
+            commit_elected(&ms->drain[wg]);
+            mbar_wait(&ms->drain[wg], 0, 2u);
+        }
+        __syncwarp();
+        // ---- results: half of the columns of its row for each thread, a quarter where both groups have the same rows
+        ms->m[wg][half][r] = m;
+        ms->l[wg][half][r] = l;
+        if (half == 0) ms->back[wg][r] = pow2_biased(vref - 6);
+        if (PAIR) {
+            group_sync();
+        } else {
+            tc_fence_before();
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            tc_fence_after();
+        }
+        float f0 = ms->back[wg][r], f1 = 0.0f;
+        l = __fadd_rn(ms->l[wg][0][r], ms->l[wg][1][r]);
+        if (!PAIR) {
+            const float ma = ms->m[0][0][r], mb = ms->m[1][0][r];
+            m = fmaxf(ma, mb);
+            const float fa = ma == -INFINITY ? 0.0f : ex2(__fsub_rn(ma, m)), fb = mb == -INFINITY ? 0.0f : ex2(__fsub_rn(mb, m));
+            l = __fmaf_rn(__fadd_rn(ms->l[0][0][r], ms->l[0][1][r]), fa, __fmul_rn(__fadd_rn(ms->l[1][0][r], ms->l[1][1][r]), fb));
+            f0 = __fmul_rn(ms->back[0][r], fa);
+            f1 = __fmul_rn(ms->back[1][r], fb);
+        }
+        const int c0 = PAIR ? half * (HDP / 2) : (2 * wg + half) * (HDP / 4), c1 = c0 + (PAIR ? HDP / 2 : HDP / 4);
         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         const int64_t grow = sq.lo + (int64_t)tok;
-        const int head = h * a.group + (row0 + r - tok * a.group);
+        const int head = h * a.group + (rb - tok * a.group);
         const int64_t si = ((int64_t)split * a.M + grow) * a.heads + head;
-        if (a.to_state && mine && half == 0) {
+        if (a.to_state && mine && c0 == 0) {
             a.out.m[si] = m;
             a.out.l[si] = l;
         }
+        const uint32_t oa = lane_addr + kOcol + (PAIR ? wg * kRows : 0);
+#pragma unroll 1
+        for (int d = c0; d < c1; d += 16) {
+            uint32_t x[16], y[16];
 #pragma unroll
-        for (int c = 0; c < HDP / 2; c += 16) {
-            uint32_t x[16];
-            if (nt > 0) {
-                tmem_ld_x16(lane_addr + kOcol + half * (HDP / 2) + c, x);
-                tc_wait_ld();
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = 0;
-            }
-            const int d = half * (HDP / 2) + c;
+            for (int k = 0; k < 16; ++k) x[k] = y[k] = 0;
+            if (nt > 0) tmem_ld_x16(oa + d, x);
+            if (!PAIR && nt > 1) tmem_ld_x16(oa + kRows + d, y);
+            wait_ld(x);
+            if (!PAIR) wait_ld(y);
             if (!mine || d >= a.c.hd) continue;
             float o[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __fmul_rn(__uint_as_float(x[i]), back);
+            for (int k = 0; k < 16; ++k) {
+                o[k] = __fmul_rn(__uint_as_float(x[k]), f0);
+                if (!PAIR) o[k] = __fmaf_rn(__uint_as_float(y[k]), f1, o[k]);
+            }
+            if (!E4M3) {  // out of the order of unpack4's pairs
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const float z = o[k + 1];
+                    o[k + 1] = o[k + 2];
+                    o[k + 2] = z;
+                }
+            }
             if (a.to_state) {
                 float4* p = reinterpret_cast<float4*>(a.out.o + si * a.c.hd + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                for (int k = 0; k < 4; ++k) p[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                 continue;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = l == 0.0f ? 0.0f : __fmul_rn(o[i], inv);
+            for (int k = 0; k < 16; ++k) o[k] = l == 0.0f ? 0.0f : __fmul_rn(o[k], inv);
             const int64_t at = grow * a.ldo + (int64_t)head * a.c.hd + d;
-            if (a.bf16) {
+            if (PARTS == 1) {
                 uint4* p = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + at);
                 uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const __nv_bfloat162 y = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&y);
+                for (int k = 0; k < 8; ++k) {
+                    const __nv_bfloat162 z = __floats2bfloat162_rn(o[2 * k], o[2 * k + 1]);
+                    w[k] = *reinterpret_cast<const uint32_t*>(&z);
                 }
                 p[0] = make_uint4(w[0], w[1], w[2], w[3]);
                 p[1] = make_uint4(w[4], w[5], w[6], w[7]);
             } else {
                 float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.o) + at);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                for (int k = 0; k < 4; ++k) p[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kSoftWarps + kConvWarps) {
+    if (warp == kSoftWarps) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
@@ -674,7 +975,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_state_join_kernel(const KvAtt
         }
         if (lo < 0) continue;
         const Rows sq = rows_of(a, lo);
-        if (sq.tiles == 0 || row >= sq.lo + (int64_t)sq.n) continue;
+        if (sq.rows == 0 || row >= sq.lo + (int64_t)sq.n) continue;
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         const int pieces = a.out.pieces + a.add.pieces;
@@ -723,28 +1024,27 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), int64_t grid, int block, size_t
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int HDP, bool E4M3, int PARTS>
-cudaError_t launch_typed(const KvAttnArgs& a, int64_t units, int splits, cudaStream_t st) {
-    auto kernel = kv_attention_tc_kernel<HDP, E4M3, PARTS>;
-    const size_t smem = kSmem<HDP, PARTS>;
+template <int HDP, bool E4M3, int PARTS, bool PAIR>
+cudaError_t launch_typed(const KvAttnArgs& a, int splits, cudaStream_t st) {
+    auto kernel = kv_attention_tc_kernel<HDP, E4M3, PARTS, PAIR>;
+    const size_t smem = kSmem<HDP, PARTS, PAIR>;
     const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
+    const int64_t units = a.M * a.group / (PAIR ? 2 * kRows : kRows) + a.batch;  // blocks of rows at most
     return launch_pdl(kernel, units * a.c.kv_heads * splits, kThreads, smem, st, a, (int)units, splits);
+}
+template <int HDP, bool E4M3>
+cudaError_t launch_code(const KvAttnArgs& a, bool pair, int splits, cudaStream_t st) {
+    if (!a.bf16) return launch_typed<HDP, E4M3, 2, false>(a, splits, st);
+    return pair ? launch_typed<HDP, E4M3, 1, true>(a, splits, st) : launch_typed<HDP, E4M3, 1, false>(a, splits, st);
 }
 
 }  // namespace
 
-int64_t kv_attn_tc_units(int64_t M, int batch, int group) { return M * group / kRows + batch; }
-
-cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, int splits, cudaStream_t st) {
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, bool pair, int splits, cudaStream_t st) {
     if (a.batch <= 0 || a.M <= 0) return cudaSuccess;
-    const int64_t units = kv_attn_tc_units(a.M, a.batch, a.group);
-    if (a.c.hd > 64) {
-        if (a.bf16) return a.c.e4m3 ? launch_typed<128, true, 1>(a, units, splits, st) : launch_typed<128, false, 1>(a, units, splits, st);
-        return a.c.e4m3 ? launch_typed<128, true, 2>(a, units, splits, st) : launch_typed<128, false, 2>(a, units, splits, st);
-    }
-    if (a.bf16) return a.c.e4m3 ? launch_typed<64, true, 1>(a, units, splits, st) : launch_typed<64, false, 1>(a, units, splits, st);
-    return a.c.e4m3 ? launch_typed<64, true, 2>(a, units, splits, st) : launch_typed<64, false, 2>(a, units, splits, st);
+    if (a.c.hd > 64) return a.c.e4m3 ? launch_code<128, true>(a, pair, splits, st) : launch_code<128, false>(a, pair, splits, st);
+    return a.c.e4m3 ? launch_code<64, true>(a, pair, splits, st) : launch_code<64, false>(a, pair, splits, st);
 }
 
 cudaError_t launch_kv_state_join(const KvAttnArgs& a, cudaStream_t st) {

@@ -53,6 +53,10 @@ struct KvAttnArgs {
     const int32_t* pages;
     int64_t ld_pages, max_pages;
     int batch, heads, group;
+    uint32_t group_mul, group_shift;
+    __device__ __forceinline__ int by_group(int n) const {  // n / group, n >= 0
+        return (int)((__umulhi((uint32_t)n, group_mul) + (uint32_t)n) >> group_shift);
+    }
     int min_rows, max_rows;  // sequences with min_rows < query rows x group <= max_rows are taken, the others left alone
     float scale_log2e;       // scale * log2(e): scores are in log2 units
     int causal;
@@ -67,10 +71,9 @@ struct KvAttnArgs {
 size_t kv_attn_part_bytes();
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st);
 
-// Many rows (kv_attention_tc.cu): the keys of a unit are cut into `splits` pieces; more than one need to_state. Blocks of
-// 128 rows that a batch can have at most; the join of out's and add's pieces into o.
-int64_t kv_attn_tc_units(int64_t M, int batch, int group);
-cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, int splits, cudaStream_t st);
+// Many rows (kv_attention_tc.cu): blocks of 128 rows, or (pair, bf16 only) of 256; their keys are cut into `splits` pieces,
+// of which more than one need to_state. The join of out's and add's pieces into o.
+cudaError_t launch_kv_attention_tc(const KvAttnArgs& a, bool pair, int splits, cudaStream_t st);
 cudaError_t launch_kv_state_join(const KvAttnArgs& a, cudaStream_t st);
 
 }  // namespace b2s
