@@ -58,9 +58,9 @@ typedef struct b2s_kv_batch {
  * for each of M rows of n_heads heads of head_dim = hd values. pos [M][n_axes] int32 (device, row stride ldpos).
  * sections (host, n_axes counts that add up to hd / 2) says how many pairs each axis turns: in blocks, axis 0's pairs
  * first, or, with interleaved != 0, dealt to the axes in turn, passing over those that have their share. The angle is
- * formed in double precision, its cosine and sine are rounded to fp32, and the result is rounded once to `type`. One
- * axis is b2s_rope_neox. y may be x; M = 0 is allowed; head_dim is even and at most 256; any row alignment that the
- * type allows. */
+ * formed and reduced in double precision, its cosine and sine are fp32 (within 1.5 * 2^-24), and the result is rounded
+ * once to `type`. One axis is b2s_rope_neox to those roundings. y may be x (other overlaps are not allowed); M = 0 is
+ * allowed; head_dim is even and at most 256; any row alignment that the type allows. */
 int b2s_rope_axes(int32_t type, const void *x, int64_t ldx, int64_t M, int n_heads, int head_dim, const int32_t *pos,
                   int64_t ldpos, int n_axes, const int32_t *sections, int interleaved, float theta_base, void *y,
                   int64_t ldy, void *stream);

@@ -70,34 +70,39 @@ def _bind():
 
 
 # ---------------------------------------------------------------------------------------------- argument checks
-def _here(t, what: str):
-    """The tensor is on the current device, where the library launches."""
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{what} must be on the current CUDA device, it is on {t.device}")
+# A call costs the host a few microseconds, most of them here: each attribute of a tensor is read once.
+_device = torch.cuda.current_device  # the device that the library launches on
 
 
-def _rows(x, width: int, what: str, dtype=None):
-    """A matrix of f32 or bf16 rows with contiguous values: (type, pointer, row stride)."""
+def _refuse_rows(x, width: int, what: str, like, dev: int):
+    if x.get_device() != dev:
+        raise ValueError(f"{what} must be on the current CUDA device, it is on {x.device}")
     if x.dim() != 2 or x.shape[1] != width or x.stride(1) != 1:
         raise ValueError(f"{what} must be a matrix with rows of {width} contiguous values, got {tuple(x.shape)} with "
                          f"strides {tuple(x.stride())}")
-    if x.dtype not in _ACT or (dtype is not None and x.dtype != dtype):
-        raise ValueError(f"{what} has dtype {x.dtype}" + (f", not {dtype}" if dtype is not None else ", not float32 or bfloat16"))
-    _here(x, what)
+    raise ValueError(f"{what} has dtype {x.dtype}" + (", not float32 or bfloat16" if like is None else ", unlike the others"))
+
+
+def _rows(x, width: int, what: str, dev: int, like=None):
+    """A matrix of f32 or bf16 rows with contiguous values: (type, rows, pointer, row stride). `like`: the type it must have."""
+    shape, stride, ty = x.shape, x.stride(), _ACT.get(x.dtype)
+    if len(shape) != 2 or shape[1] != width or stride[1] != 1 or ty is None or (like is not None and ty != like) or \
+            x.get_device() != dev:
+        _refuse_rows(x, width, what, like, dev)
     # a single row may have any stride: it is never used
-    return _ACT[x.dtype], x.data_ptr(), x.stride(0) if x.shape[0] > 1 else width
+    return ty, shape[0], x.data_ptr(), stride[0] if shape[0] > 1 else width
 
 
-def _ints(t, dtype, shape, what: str) -> int:
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    _here(t, what)
+def _ints(t, dtype, shape, what: str, dev: int) -> int:
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on the current CUDA device, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _stream(stream) -> int:
+def _stream(stream, dev: int) -> int:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return torch.cuda.current_stream(dev).cuda_stream
     return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -122,6 +127,7 @@ class Cache:
                                   v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self.ref = C.addressof(self.struct)
         self.width = self.n_kv_heads * self.head_dim
+        self.device = k.get_device()
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, dtype=torch.int8, device="cuda"):
@@ -139,10 +145,12 @@ class Batch:
         b = kv_len.shape[0]
         if pages.dim() != 2 or pages.shape[0] != b or pages.dtype != torch.int32 or (pages.shape[1] > 1 and pages.stride(1) != 1):
             raise ValueError(f"pages must be an int32 matrix of {b} rows, got {pages.dtype} {tuple(pages.shape)}")
-        _here(pages, "pages")
+        dev = _device()
+        if pages.get_device() != dev:
+            raise ValueError(f"pages must be on the current CUDA device, it is on {pages.device}")
         self.q_start, self.kv_len, self.pages, self.max_q = q_start, kv_len, pages, int(max_q)
-        self.struct = BatchStruct(b, self.max_q, _ints(q_start, torch.int32, (b + 1,), "q_start"),
-                                  _ints(kv_len, torch.int32, (b,), "kv_len"), pages.data_ptr(), pages.shape[1],
+        self.struct = BatchStruct(b, self.max_q, _ints(q_start, torch.int32, (b + 1,), "q_start", dev),
+                                  _ints(kv_len, torch.int32, (b,), "kv_len", dev), pages.data_ptr(), pages.shape[1],
                                   pages.stride(0) if b > 1 else pages.shape[1])
         self.ref = C.addressof(self.struct)
 
@@ -152,40 +160,41 @@ def rope_axes(x, n_heads: int, head_dim: int, pos, sections, theta_base: float, 
               stream=None) -> None:
     """Rotates rows of n_heads heads (NEOX pairs) by positions pos [M, axes] int32; sections[a] pairs turn by axis a, in
     blocks or dealt in turn (interleaved). y may be x."""
-    width = n_heads * head_dim
-    ty, px, ldx = _rows(x, width, "x")
-    _, py, ldy = _rows(y, width, "y", x.dtype)
+    width, dev = n_heads * head_dim, _device()
+    ty, M, px, ldx = _rows(x, width, "x", dev)
+    _, My, py, ldy = _rows(y, width, "y", dev, ty)
     n = len(sections)
-    if y.shape[0] != x.shape[0] or px == py and x.stride(0) != y.stride(0):
+    if My != M or px == py and ldx != ldy:
         raise ValueError("x and y must have the same rows")
-    pp = _ints(pos, torch.int32, (x.shape[0], n), "pos")
-    check(_bind().b2s_rope_axes(ty, px, ldx, x.shape[0], n_heads, head_dim, pp, n, n, (C.c_int32 * n)(*sections),
-                                int(interleaved), theta_base, py, ldy, _stream(stream)))
+    pp = _ints(pos, torch.int32, (M, n), "pos", dev)
+    check(_bind().b2s_rope_axes(ty, px, ldx, M, n_heads, head_dim, pp, n, n, (C.c_int32 * n)(*sections), int(interleaved),
+                                theta_base, py, ldy, _stream(stream, dev)))
 
 
 def write(cache: Cache, k, v, slots, stream=None) -> None:
     """Quantises rows of keys and values [M, n_kv_heads * head_dim] into slots [M] int64 (negative: skipped)."""
-    ty, pk, ldk = _rows(k, cache.width, "k")
-    _, pv, ldv = _rows(v, cache.width, "v", k.dtype)
-    if v.shape[0] != k.shape[0]:
-        raise ValueError("k and v must have the same rows")
-    _here(cache.k, "cache")
-    check(_bind().b2s_kv_write(cache.ref, ty, pk, ldk, pv, ldv, k.shape[0],
-                               _ints(slots, torch.int64, (k.shape[0],), "slots"), _stream(stream)))
+    dev = _device()
+    ty, M, pk, ldk = _rows(k, cache.width, "k", dev)
+    _, Mv, pv, ldv = _rows(v, cache.width, "v", dev, ty)
+    if Mv != M or cache.device != dev:
+        raise ValueError("k, v and the cache must have the same rows and device")
+    check(_bind().b2s_kv_write(cache.ref, ty, pk, ldk, pv, ldv, M, _ints(slots, torch.int64, (M,), "slots", dev),
+                               _stream(stream, dev)))
 
 
 def read(cache: Cache, slots, k=None, v=None, stream=None) -> None:
     """Reads slots [M] int64 back into rows k and / or v (zeros for a negative slot)."""
-    M = slots.shape[0]
-    ty, pk, ldk, pv, ldv = TYPE_F32, None, 0, None, 0
+    dev = _device()
+    ty, M, pk, ldk, pv, ldv = None, slots.shape[0], None, 0, None, 0
+    Mk = Mv = M
     if k is not None:
-        ty, pk, ldk = _rows(k, cache.width, "k")
+        ty, Mk, pk, ldk = _rows(k, cache.width, "k", dev)
     if v is not None:
-        ty, pv, ldv = _rows(v, cache.width, "v", None if k is None else k.dtype)
-    if any(t is not None and t.shape[0] != M for t in (k, v)):
-        raise ValueError(f"k and v must have {M} rows")
-    _here(cache.k, "cache")
-    check(_bind().b2s_kv_read(cache.ref, _ints(slots, torch.int64, (M,), "slots"), M, ty, pk, ldk, pv, ldv, _stream(stream)))
+        ty, Mv, pv, ldv = _rows(v, cache.width, "v", dev, ty)
+    if Mk != M or Mv != M or cache.device != dev:
+        raise ValueError(f"k and v must have {M} rows and the cache's device")
+    check(_bind().b2s_kv_read(cache.ref, _ints(slots, torch.int64, (M,), "slots", dev), M, TYPE_F32 if ty is None else ty, pk,
+                              ldk, pv, ldv, _stream(stream, dev)))
 
 
 def attention_workspace_size(cache: Cache, batch: Batch, M: int, n_heads: int, prefix_len: int = 0) -> int:
@@ -193,34 +202,33 @@ def attention_workspace_size(cache: Cache, batch: Batch, M: int, n_heads: int, p
     return int(_bind().b2s_attention_kv_workspace_size(cache.ref, batch.ref, M, n_heads, prefix_len))
 
 
-def _qo(cache, q, o, n_heads, workspace):
+def _qo(cache, q, o, n_heads, workspace, dev):
     width = n_heads * cache.head_dim
-    ty, pq, ldq = _rows(q, width, "q")
-    _, po, ldo = _rows(o, width, "o", q.dtype)
-    if o.shape[0] != q.shape[0]:
+    ty, M, pq, ldq = _rows(q, width, "q", dev)
+    _, Mo, po, ldo = _rows(o, width, "o", dev, ty)
+    if Mo != M:
         raise ValueError("q and o must have the same rows")
-    if not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
-    _here(cache.k, "cache")
-    _here(workspace, "workspace")
-    return ty, pq, ldq, po, ldo
+    if cache.device != dev or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("the cache and a contiguous workspace must be on the current CUDA device")
+    return ty, M, pq, ldq, po, ldo
 
 
 def attention(cache: Cache, batch: Batch, q, n_heads: int, scale: float, causal: bool, o, workspace, stream=None) -> None:
     """o = softmax(scale q K^T) V of each sequence's query rows over its cached tokens (its last tokens, if causal)."""
-    ty, pq, ldq, po, ldo = _qo(cache, q, o, n_heads, workspace)
-    check(_bind().b2s_attention_kv(cache.ref, batch.ref, ty, pq, ldq, q.shape[0], n_heads, scale, int(bool(causal)), po, ldo,
-                                   workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream)))
+    dev = _device()
+    ty, M, pq, ldq, po, ldo = _qo(cache, q, o, n_heads, workspace, dev)
+    check(_bind().b2s_attention_kv(cache.ref, batch.ref, ty, pq, ldq, M, n_heads, scale, int(bool(causal)), po, ldo,
+                                   workspace.data_ptr(), workspace.nbytes, _stream(stream, dev)))
 
 
 def attention_prefix(cache: Cache, batch: Batch, prefix_pages, prefix_len: int, q, n_heads: int, scale: float,
                      causal: bool, o, workspace, stream=None) -> None:
     """attention() with prefix_len tokens in prefix_pages [pages] int32 in front of every sequence."""
-    ty, pq, ldq, po, ldo = _qo(cache, q, o, n_heads, workspace)
-    need = -(-prefix_len // cache.page_size)
-    if prefix_pages.dim() != 1 or prefix_pages.shape[0] < need:
-        raise ValueError(f"prefix_pages must hold {need} pages")
-    pp = _ints(prefix_pages, torch.int32, tuple(prefix_pages.shape), "prefix_pages")
-    check(_bind().b2s_attention_kv_prefix(cache.ref, batch.ref, pp, prefix_len, ty, pq, ldq, q.shape[0], n_heads, scale,
-                                          int(bool(causal)), po, ldo, workspace.data_ptr(),
-                                          workspace.numel() * workspace.element_size(), _stream(stream)))
+    dev = _device()
+    ty, M, pq, ldq, po, ldo = _qo(cache, q, o, n_heads, workspace, dev)
+    if prefix_pages.dim() != 1 or prefix_pages.shape[0] * cache.page_size < prefix_len:
+        raise ValueError(f"prefix_pages must hold the pages of {prefix_len} tokens")
+    pp = _ints(prefix_pages, torch.int32, prefix_pages.shape, "prefix_pages", dev)
+    check(_bind().b2s_attention_kv_prefix(cache.ref, batch.ref, pp, prefix_len, ty, pq, ldq, M, n_heads, scale,
+                                          int(bool(causal)), po, ldo, workspace.data_ptr(), workspace.nbytes,
+                                          _stream(stream, dev)))

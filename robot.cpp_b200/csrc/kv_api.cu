@@ -241,8 +241,8 @@ int b2s_rope_axes(int32_t type, const void* x, int64_t ldx, int64_t M, int n_hea
     if (!sections || (M > 0 && (!x || !y || !pos)))
         return fail(B2S_ERR_INVALID_ARG, "rope_axes: x, y, pos and sections must be non-NULL");
     if (M < 0 || n_heads <= 0 || head_dim <= 0 || head_dim % 2) return fail(B2S_ERR_INVALID_ARG, "rope_axes: bad shape");
-    if (head_dim > 256 || n_heads > 65535 || M > kMaxInt)
-        return fail(B2S_ERR_UNSUPPORTED, "rope_axes: head_dim up to 256, n_heads up to 65535 and M below 2^31");
+    if (head_dim > 256 || M > kMaxInt / n_heads)
+        return fail(B2S_ERR_UNSUPPORTED, "rope_axes: head_dim up to 256 and M x n_heads below 2^31");
     const int64_t width = (int64_t)n_heads * head_dim;
     if (ldx < width || ldy < width) return fail(B2S_ERR_INVALID_ARG, "rope_axes: row stride below n_heads * head_dim");
     if (!aligned(x, size_of(type)) || !aligned(y, size_of(type)))
@@ -261,12 +261,16 @@ int b2s_rope_axes(int32_t type, const void* x, int64_t ldx, int64_t M, int n_hea
     const int half = head_dim / 2;
     int left[4] = {0, 0, 0, 0};
     for (int i = 0; i < n_axes; ++i) left[i] = sections[i];
+    // theta_base^(-2 i / hd) / pi by repeated products in extended precision (their errors stay far below a double's step)
+    const long double ratio = std::pow((long double)theta_base, -2.0L / head_dim);
+    long double turn = 1.0L / 3.14159265358979323846264338L;
     for (int i = 0, ax = 0; i < half; ++i) {
         while (left[ax] == 0) ax = (ax + 1) % n_axes;
         p.axis[i] = (uint8_t)ax;
         --left[ax];
         if (interleaved) ax = (ax + 1) % n_axes;
-        p.turn[i] = std::pow((double)theta_base, -2.0 * i / head_dim) / 3.14159265358979323846;
+        p.turn[i] = (double)turn;
+        turn *= ratio;
     }
     if ((rc = b2s_device_check())) return rc;
     return launched(b2s::launch_rope_axes(type == B2S_TYPE_BF16, x, ldx, M, n_heads, head_dim, pos, ldpos, p, y, ldy,
@@ -280,7 +284,8 @@ int b2s_kv_write(const b2s_kv_cache* cache, int32_t type, const void* k, int64_t
     int rc;
     if ((rc = cache_view(cache, &c, "kv_write"))) return rc;
     if ((rc = check_type(type, "kv_write"))) return rc;
-    if (M < 0 || M > kMaxInt) return fail(B2S_ERR_INVALID_ARG, "kv_write: bad M");
+    if (M < 0) return fail(B2S_ERR_INVALID_ARG, "kv_write: M is negative");
+    if (M > kMaxInt / c.kv_heads) return fail(B2S_ERR_UNSUPPORTED, "kv_write: M x n_kv_heads has to be below 2^31");
     if (M > 0 && !slots) return fail(B2S_ERR_INVALID_ARG, "kv_write: slots is NULL");
     const int64_t width = (int64_t)c.kv_heads * c.hd;
     if ((rc = check_rows(k, M, ldk, width, type, "kv_write", "k"))) return rc;
@@ -296,7 +301,8 @@ int b2s_kv_read(const b2s_kv_cache* cache, const int64_t* slots, int64_t M, int3
     int rc;
     if ((rc = cache_view(cache, &c, "kv_read"))) return rc;
     if ((rc = check_type(type, "kv_read"))) return rc;
-    if (M < 0 || M > kMaxInt) return fail(B2S_ERR_INVALID_ARG, "kv_read: bad M");
+    if (M < 0) return fail(B2S_ERR_INVALID_ARG, "kv_read: M is negative");
+    if (M > kMaxInt / c.kv_heads) return fail(B2S_ERR_UNSUPPORTED, "kv_read: M x n_kv_heads has to be below 2^31");
     if (M > 0 && !slots) return fail(B2S_ERR_INVALID_ARG, "kv_read: slots is NULL");
     if (M > 0 && !k && !v) return fail(B2S_ERR_INVALID_ARG, "kv_read: k and v are both NULL");
     const int64_t width = (int64_t)c.kv_heads * c.hd;

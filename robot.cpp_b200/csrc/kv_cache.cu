@@ -25,211 +25,336 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStre
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Four consecutive values; the address is aligned to four of them.
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                       __uint_as_float(u.y & 0xffff0000u));
+// Eight consecutive values; the address is aligned to 16 bytes.
+struct F8 {
+    float v[8];
+};
+__device__ __forceinline__ F8 load8(const float* p) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
-__device__ __forceinline__ void store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-    uint2 u;
-    u.x = *reinterpret_cast<const uint32_t*>(&a);
-    u.y = *reinterpret_cast<const uint32_t*>(&b);
-    *reinterpret_cast<uint2*>(p) = u;
+__device__ __forceinline__ F8 load8(const __nv_bfloat16* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    F8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.v[2 * i] = __uint_as_float(w[i] << 16);
+        r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+    return r;
+}
+__device__ __forceinline__ void store8(float* p, const F8& x) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const F8& x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(x.v[2 * i], x.v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ------------------------------------------------------------------------------------------------ rotary positions
-constexpr int kRopeRows = 4, kRopeThreads = 256, kRopeHalf = 128;
+__device__ __forceinline__ uint4 pack16(const float (&v)[4]) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint4 pack16(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void unpack16(uint4 u, float (&v)[4]) {
+    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack16(uint4 u, float (&v)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
 
-// A block turns kRopeRows rows' heads [h0, h1): the rows' cosines and sines go to shared memory once and serve every
-// head, so the double-precision angles cost hd / 2 per row and not per head. The angle is kept in units of pi: its
-// reduction is then exact.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads)
-rope_axes_kernel(const T* x, int64_t ldx, int64_t M, int n_heads, int hd, const int32_t* __restrict__ pos, int64_t ldpos,
-                 const __grid_constant__ RopePairs pairs, T* y, int64_t ldy, int heads_per_block) {
+// Cosine and sine of pos * turn (units of pi). The product and its reduction to [-1, 1] are double, the reduction is exact;
+// the remainder goes on as a float and its rest r, with sin(h + r) = sin h + r cos h. Each is within 1.5 * 2^-24 (the float
+// functions' one unit in the last place, then one rounding). In double throughout the functions took as long as the rows.
+__device__ __forceinline__ float2 cos_sin(int pos, double turn) {
+    const double t = (double)pos * turn, r = t - 2.0 * rint(0.5 * t);
+    const float h = (float)r, l = (float)(r - (double)h) * 3.14159265f;
+    float s, c;
+    sincospif(h, &s, &c);
+    return make_float2(__fmaf_rn(-l, s, c), __fmaf_rn(l, c, s));
+}
+
+// A warp turns one row's heads [h0, h0 + heads): per_head lanes of W pairs (16 bytes and the 16 half a head on) hold their
+// cosines and sines in registers for all of them, 32 / per_head heads side by side, kRopeFlight of those steps in flight; the
+// angles are formed while the first ones arrive.
+constexpr int kRopeFlight = 4;
+template <typename T, int W>
+__global__ void __launch_bounds__(256)
+rope_axes_kernel(const T* x, int64_t ldx, int M, int n_heads, int hd, const int32_t* __restrict__ pos, int64_t ldpos,
+                 const __grid_constant__ RopePairs pairs, T* y, int64_t ldy, int heads_per_warp, int warps_a_row) {
+    const int half = hd / 2, per_head = half / W, G = 32 / per_head;
+    const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), row = w / (uint32_t)warps_a_row;
+    const int lane = threadIdx.x & 31, g = lane / per_head, i = (lane - g * per_head) * W;
+    const int h0 = (int)(w - row * (uint32_t)warps_a_row) * heads_per_warp, h1 = min(n_heads, h0 + heads_per_warp);
+    griddep_wait();
+    griddep_launch();
+    if (row >= (uint32_t)M || g >= G) return;
+    const T* xr = x + row * ldx + i;
+    T* yr = y + row * ldy + i;
+    float2 cs[W];
+    bool angles = false;
+    for (int h = h0 + g; h < h1; h += G * kRopeFlight) {
+        uint4 a[kRopeFlight], b[kRopeFlight];
+#pragma unroll
+        for (int k = 0; k < kRopeFlight; ++k) {
+            const int64_t at = (int64_t)min(h + k * G, h1 - 1) * hd;  // past the end the last head once more, not written
+            a[k] = *reinterpret_cast<const uint4*>(xr + at);
+            b[k] = *reinterpret_cast<const uint4*>(xr + at + half);
+        }
+        if (!angles) {
+            angles = true;
+#pragma unroll
+            for (int j = 0; j < W; ++j) cs[j] = cos_sin(pos[row * ldpos + pairs.axis[i + j]], pairs.turn[i + j]);
+        }
+#pragma unroll
+        for (int k = 0; k < kRopeFlight; ++k) {
+            if (h + k * G >= h1) break;
+            float u[W], v[W], p[W], q[W];
+            unpack16(a[k], u);
+            unpack16(b[k], v);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                p[j] = __fsub_rn(__fmul_rn(u[j], cs[j].x), __fmul_rn(v[j], cs[j].y));
+                q[j] = __fadd_rn(__fmul_rn(u[j], cs[j].y), __fmul_rn(v[j], cs[j].x));
+            }
+            const int64_t at = (int64_t)(h + k * G) * hd;
+            *reinterpret_cast<uint4*>(yr + at) = pack16(p);
+            *reinterpret_cast<uint4*>(yr + at + half) = pack16(q);
+        }
+    }
+}
+
+// Any alignment and any half: one pair a thread and step, cosines and sines of a block's rows in shared memory.
+constexpr int kRopeRows = 4, kRopeHalf = 128;
+template <typename T>
+__global__ void __launch_bounds__(256)
+rope_axes_any_kernel(const T* x, int64_t ldx, int64_t M, int n_heads, int hd, const int32_t* __restrict__ pos, int64_t ldpos,
+                     const __grid_constant__ RopePairs pairs, T* y, int64_t ldy) {
     __shared__ float2 cs[kRopeRows][kRopeHalf];
     const int half = hd / 2;
     const int64_t m0 = (int64_t)blockIdx.x * kRopeRows;
     const int rows = (int)min((int64_t)kRopeRows, M - m0);
     griddep_wait();
     griddep_launch();
-    for (int e = threadIdx.x; e < rows * half; e += kRopeThreads) {
+    for (int e = threadIdx.x; e < rows * half; e += 256) {
         const int r = e / half, i = e - r * half;
-        double s, c;
-        sincospi((double)pos[(m0 + r) * ldpos + pairs.axis[i]] * pairs.turn[i], &s, &c);
-        cs[r][i] = make_float2((float)c, (float)s);
+        cs[r][i] = cos_sin(pos[(m0 + r) * ldpos + pairs.axis[i]], pairs.turn[i]);
     }
     __syncthreads();
-    const int h0 = blockIdx.y * heads_per_block, h1 = min(n_heads, h0 + heads_per_block);
-    const int step = VEC ? 4 : 1, per_head = half / step, per_row = (h1 - h0) * per_head;
-    for (int e = threadIdx.x; e < rows * per_row; e += kRopeThreads) {
-        const int r = e / per_row, f = e - r * per_row, h = f / per_head, i = (f - h * per_head) * step;
-        const T* xp = x + (m0 + r) * ldx + (int64_t)(h0 + h) * hd + i;
-        T* yp = y + (m0 + r) * ldy + (int64_t)(h0 + h) * hd + i;
-        if (VEC) {
-            const float4 a = load4(xp), b = load4(xp + half);
-            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-            float u[4], w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 t = cs[r][i + j];
-                u[j] = __fsub_rn(__fmul_rn(av[j], t.x), __fmul_rn(bv[j], t.y));
-                w[j] = __fadd_rn(__fmul_rn(av[j], t.y), __fmul_rn(bv[j], t.x));
-            }
-            store4(yp, make_float4(u[0], u[1], u[2], u[3]));
-            store4(yp + half, make_float4(w[0], w[1], w[2], w[3]));
-        } else {
-            const float a = (float)xp[0], b = (float)xp[half];
+    const int per_row = n_heads * half;
+    for (int r = 0; r < rows; ++r) {
+        for (int e = threadIdx.x; e < per_row; e += 256) {
+            const int h = e / half, i = e - h * half;
+            const T* p = x + (m0 + r) * ldx + (int64_t)h * hd + i;
+            T* q = y + (m0 + r) * ldy + (int64_t)h * hd + i;
+            const float a = (float)p[0], b = (float)p[half];
             const float2 t = cs[r][i];
-            yp[0] = (T)__fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
-            yp[half] = (T)__fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
+            q[0] = (T)__fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
+            q[half] = (T)__fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ quantised write
-// Code of p = x * (TOP / a).
+// Codes of eight x * s, packed.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t code_of(float p) {
-    if (E4M3) return (uint32_t)__nv_cvt_float_to_fp8(p, __NV_SATFINITE, __NV_E4M3);
-    return (uint32_t)(int)fminf(fmaxf(roundf(p), -127.0f), 127.0f) & 0xffu;
+__device__ __forceinline__ uint2 codes_of(const F8& x, float s) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __fmul_rn(x.v[4 * i + j], s);
+        if (E4M3) {
+            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(p[0], p[1]), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(p[2], p[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        } else {
+            w[i] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)(int)fminf(fmaxf(roundf(p[j]), -127.0f), 127.0f) & 0xffu) << (8 * j);
+        }
+    }
+    return make_uint2(w[0], w[1]);
 }
 
-// Lanes of a group share one (token, head, key or value): four values each, so a head of 128 is a warp's 512 bytes.
-// Items are ordered (token, key or value, head): consecutive groups read consecutive memory.
+// LANES lanes share one (token, key or value, head), eight values each. A warp takes kFlight heads for each of its 32 / LANES
+// groups from one token's 2 kv_heads: all loads are in flight before the first is used.
+constexpr int kFlight = 4;
 template <typename T, bool E4M3, int LANES>
 __global__ void __launch_bounds__(256)
-kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv, int64_t M,
-                const int64_t* __restrict__ slots) {
-    const int lane = threadIdx.x % LANES, d = 4 * lane;
-    const int64_t groups = (int64_t)gridDim.x * (256 / LANES);
-    const int64_t items = M * 2 * c.kv_heads, n_slots = c.n_pages << c.page_shift;
-    const bool on = d < c.hd;
+kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv, int M,
+                const int64_t* __restrict__ slots, int warps_a_token) {
+    constexpr int G = 32 / LANES;
+    const int lane = threadIdx.x % LANES, g = (threadIdx.x & 31) / LANES, d = 8 * lane;
+    const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), token = w / (uint32_t)warps_a_token;
+    const int64_t m = token;
+    // heads f0, f0 + step, ...: a token's warps have the same number of them
+    const int f0 = (int)(w - token * (uint32_t)warps_a_token) * G + g, step = warps_a_token * G, heads = 2 * c.kv_heads;
     griddep_wait();
     griddep_launch();
-    for (int64_t it = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; it < (items + groups - 1) / groups * groups;
-         it += groups) {
-        const int64_t m = it / (2 * c.kv_heads);
-        const int f = (int)(it - m * 2 * c.kv_heads), is_v = f >= c.kv_heads, h = f - is_v * c.kv_heads;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        int64_t slot = -1;
-        if (it < items) {
-            slot = slots[m];
-            if (on) x = load4((is_v ? v + m * ldv : k + m * ldk) + (int64_t)h * c.hd + d);
-        }
-        float a = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-        // an infinity or a NaN anywhere: x - x is NaN for both
-        const float z = (x.x - x.x) + (x.y - x.y) + (x.z - x.z) + (x.w - x.w);
-        if (z != 0.0f) a = INFINITY;
+    if (m >= M) return;
+    const int64_t slot = slots[m];  // looked at when the rows are on their way
+    F8 x[kFlight];
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        if (slot < 0) continue;
-        if (slot >= n_slots) {
-            if (lane == 0) atomicOr(&g_device_error, kErrIndex);
-            continue;
-        }
-        const float top = E4M3 ? 448.0f : 127.0f;
-        const bool bad = a == INFINITY;
-        a = fmaxf(a, 0x1p-100f);
-        const float s = bad ? 0.0f : __fdiv_rn(top, a);
-        uint32_t w = 0;
-        if (!bad)
-            w = code_of<E4M3>(__fmul_rn(x.x, s)) | code_of<E4M3>(__fmul_rn(x.y, s)) << 8 |
-                code_of<E4M3>(__fmul_rn(x.z, s)) << 16 | code_of<E4M3>(__fmul_rn(x.w, s)) << 24;
-        const int64_t row = (((slot >> c.page_shift) * c.kv_heads + h) << c.page_shift) + (slot & ((1 << c.page_shift) - 1));
-        if (on) *reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + row * c.hd + d) = w;
-        if (lane == 0) (is_v ? c.vs : c.ks)[row] = bad ? __int_as_float(0x7fc00000) : __fdiv_rn(a, top);
+    for (int i = 0; i < kFlight; ++i) {
+        const int f = f0 + i * step;
+        if (f < heads && d < c.hd)
+            x[i] = load8(f < c.kv_heads ? k + m * ldk + (int64_t)f * c.hd + d : v + m * ldv + (int64_t)(f - c.kv_heads) * c.hd + d);
+        else
+            x[i] = F8{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+    }
+    if (slot < 0) return;
+    if (slot >= c.n_pages << c.page_shift) {
+        if (f0 == 0 && lane == 0) atomicOr(&g_device_error, kErrIndex);
+        return;
+    }
+    const int64_t row0 = (((slot >> c.page_shift) * c.kv_heads) << c.page_shift) + (slot & ((1 << c.page_shift) - 1));
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+        const int f = f0 + i * step;
+        uint32_t bits = 0;  // of the largest |x|; an infinity or a NaN is 0x7f800000 or more
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(x[i].v[j]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+        if (f >= heads) continue;
+        constexpr float top = E4M3 ? 448.0f : 127.0f, by_top = 1.0f / top;
+        const bool bad = bits >= 0x7f800000u;
+        const float a = bad ? 1.0f : fmaxf(__uint_as_float(bits), 0x1p-100f);
+        uint2 codes = codes_of<E4M3>(x[i], __fdiv_rn(top, a));
+        if (bad) codes = make_uint2(0, 0);
+        // a / top, correctly rounded: the quotient by the rounded reciprocal, corrected once by its exact remainder
+        const float q0 = __fmul_rn(a, by_top), quotient = __fmaf_rn(__fmaf_rn(-q0, top, a), by_top, q0);
+        const bool is_v = f >= c.kv_heads;
+        const int64_t row = row0 + ((int64_t)(is_v ? f - c.kv_heads : f) << c.page_shift);
+        if (d < c.hd) *reinterpret_cast<uint2*>((is_v ? c.v : c.k) + row * c.hd + d) = codes;
+        if (lane == 0) (is_v ? c.vs : c.ks)[row] = bad ? __int_as_float(0x7fc00000) : quotient;
     }
 }
 
 // ------------------------------------------------------------------------------------------------ read back
 template <bool E4M3>
-__device__ __forceinline__ float4 values_of(uint32_t w) {
-    if (E4M3) {
-        const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3));
-        const __half2 b = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3));
-        const float2 x = __half22float2(a), y = __half22float2(b);
-        return make_float4(x.x, x.y, y.x, y.y);
+__device__ __forceinline__ F8 values_of(uint2 u, float s) {
+    F8 r;
+    const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (E4M3) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> (16 * j) & 0xffffu), __NV_E4M3));
+                const float2 f = __half22float2(a);
+                r.v[4 * i + 2 * j] = __fmul_rn(f.x, s);
+                r.v[4 * i + 2 * j + 1] = __fmul_rn(f.y, s);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.v[4 * i + j] = __fmul_rn((float)(int8_t)(w[i] >> (8 * j) & 0xffu), s);
+        }
     }
-    return make_float4((float)(int8_t)(w & 0xff), (float)(int8_t)((w >> 8) & 0xff), (float)(int8_t)((w >> 16) & 0xff),
-                       (float)(int8_t)(w >> 24));
+    return r;
 }
 
+// As the write: a warp takes kFlight heads a group from one token. `parts` = 2: keys and values, 1: the one whose rows are given.
 template <typename T, bool E4M3, int LANES>
 __global__ void __launch_bounds__(256)
-kv_read_kernel(KvView c, const int64_t* __restrict__ slots, int64_t M, T* __restrict__ k, int64_t ldk, T* __restrict__ v,
-               int64_t ldv) {
-    const int lane = threadIdx.x % LANES, d = 4 * lane;
-    if (d >= c.hd) return;
-    const int parts = (k ? 1 : 0) + (v ? 1 : 0);
-    const int64_t groups = (int64_t)gridDim.x * (256 / LANES);
-    const int64_t items = M * parts * c.kv_heads, n_slots = c.n_pages << c.page_shift;
+kv_read_kernel(KvView c, const int64_t* __restrict__ slots, int M, T* __restrict__ k, int64_t ldk, T* __restrict__ v, int64_t ldv,
+               int parts, int warps_a_token) {
+    constexpr int G = 32 / LANES;
+    const int lane = threadIdx.x % LANES, g = (threadIdx.x & 31) / LANES, d = 8 * lane;
+    const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), token = w / (uint32_t)warps_a_token;
+    const int64_t m = token;
+    const int f0 = (int)(w - token * (uint32_t)warps_a_token) * G + g, step = warps_a_token * G, heads = parts * c.kv_heads;
     griddep_wait();
     griddep_launch();
-    for (int64_t it = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; it < items; it += groups) {
-        const int64_t m = it / (parts * c.kv_heads);
-        const int f = (int)(it - m * parts * c.kv_heads), second = f >= c.kv_heads, h = f - second * c.kv_heads;
-        const bool is_v = !k || second;
-        const int64_t slot = slots[m];
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (slot >= n_slots) {
-            if (lane == 0) atomicOr(&g_device_error, kErrIndex);
-        } else if (slot >= 0) {
-            const int64_t row =
-                (((slot >> c.page_shift) * c.kv_heads + h) << c.page_shift) + (slot & ((1 << c.page_shift) - 1));
-            const float s = (is_v ? c.vs : c.ks)[row];
-            x = values_of<E4M3>(*reinterpret_cast<const uint32_t*>((is_v ? c.v : c.k) + row * c.hd + d));
-            x = make_float4(__fmul_rn(x.x, s), __fmul_rn(x.y, s), __fmul_rn(x.z, s), __fmul_rn(x.w, s));
+    if (m >= M || d >= c.hd) return;
+    const int64_t slot = slots[m];
+    const bool there = slot >= 0 && slot < c.n_pages << c.page_shift;
+    if (slot >= 0 && !there && f0 == 0 && lane == 0) atomicOr(&g_device_error, kErrIndex);
+    const int64_t row0 =
+        there ? (((slot >> c.page_shift) * c.kv_heads) << c.page_shift) + (slot & ((1 << c.page_shift) - 1)) : 0;
+    uint2 u[kFlight];
+    float s[kFlight];
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+        const int f = f0 + i * step;
+        u[i] = make_uint2(0, 0);
+        s[i] = 0.0f;
+        if (there && f < heads) {
+            const bool is_v = !k || f >= c.kv_heads;
+            const int64_t row = row0 + ((int64_t)(f >= c.kv_heads ? f - c.kv_heads : f) << c.page_shift);
+            u[i] = *reinterpret_cast<const uint2*>((is_v ? c.v : c.k) + row * c.hd + d);
+            s[i] = (is_v ? c.vs : c.ks)[row];
         }
-        store4((is_v ? v + m * ldv : k + m * ldk) + (int64_t)h * c.hd + d, x);
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+        const int f = f0 + i * step;
+        if (f >= heads) break;
+        const bool is_v = !k || f >= c.kv_heads;
+        const int h = f >= c.kv_heads ? f - c.kv_heads : f;
+        F8 x = values_of<E4M3>(u[i], s[i]);
+        if (!there) x = F8{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
+        store8((is_v ? v + m * ldv : k + m * ldk) + (int64_t)h * c.hd + d, x);
     }
 }
-
-constexpr int64_t kBlocks = 148 * 8;  // 8 blocks of 256 threads fill an SM
 
 template <typename T>
 cudaError_t rope_typed(const void* x, int64_t ldx, int64_t M, int n_heads, int hd, const int32_t* pos, int64_t ldpos,
                        const RopePairs& pairs, void* y, int64_t ldy, cudaStream_t st) {
-    const int64_t blocks = ceil_div(M, kRopeRows);
-    // Few rows: split the heads as well, until the grid has two blocks for each SM.
-    int split = (int)ceil_div(2 * 148, blocks);
-    if (split > n_heads) split = n_heads;
-    const int per = (int)ceil_div(n_heads, split);
-    const dim3 grid((unsigned)blocks, (unsigned)ceil_div(n_heads, per));
-    const size_t a4 = 4 * sizeof(T) - 1;
-    const bool vec = (hd / 2) % 4 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & a4) == 0 &&
-                     ldx % 4 == 0 && ldy % 4 == 0;
-    if (vec)
-        return launch_pdl(rope_axes_kernel<T, true>, grid, dim3(kRopeThreads), st, static_cast<const T*>(x), ldx, M, n_heads,
-                          hd, pos, ldpos, pairs, static_cast<T*>(y), ldy, per);
-    return launch_pdl(rope_axes_kernel<T, false>, grid, dim3(kRopeThreads), st, static_cast<const T*>(x), ldx, M, n_heads, hd,
-                      pos, ldpos, pairs, static_cast<T*>(y), ldy, per);
+    constexpr int W = 16 / sizeof(T);
+    const bool wide = (hd / 2) % W == 0 && hd / 2 / W <= 32 &&
+                      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0 && ldx % W == 0 && ldy % W == 0;
+    if (!wide)
+        return launch_pdl(rope_axes_any_kernel<T>, dim3((unsigned)ceil_div(M, kRopeRows)), dim3(256), st, static_cast<const T*>(x),
+                          ldx, M, n_heads, hd, pos, ldpos, pairs, static_cast<T*>(y), ldy);
+    // A warp takes all of a row's heads, which share its angles; with few rows, one step in flight of them.
+    const int step = 32 / (hd / 2 / W) * kRopeFlight, per = M >= 16 * 148 || n_heads < step ? n_heads : step;
+    const int warps = (int)ceil_div(n_heads, per);
+    return launch_pdl(rope_axes_kernel<T, W>, dim3((unsigned)ceil_div(M * warps, 8)), dim3(256), st, static_cast<const T*>(x), ldx,
+                      (int)M, n_heads, hd, pos, ldpos, pairs, static_cast<T*>(y), ldy, per, warps);
 }
 
 template <typename T, bool E4M3, int LANES>
 cudaError_t write_typed(const KvView& c, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t M,
                         const int64_t* slots, cudaStream_t st) {
-    const int64_t b = ceil_div(M * 2 * c.kv_heads, 256 / LANES);
-    return launch_pdl(kv_write_kernel<T, E4M3, LANES>, dim3((unsigned)(b < kBlocks ? b : kBlocks)), dim3(256), st, c,
-                      static_cast<const T*>(k), ldk, static_cast<const T*>(v), ldv, M, slots);
+    const int per = (int)ceil_div(2 * c.kv_heads, kFlight * (32 / LANES));
+    return launch_pdl(kv_write_kernel<T, E4M3, LANES>, dim3((unsigned)ceil_div(M * per, 8)), dim3(256), st, c,
+                      static_cast<const T*>(k), ldk, static_cast<const T*>(v), ldv, (int)M, slots, per);
 }
 template <typename T, bool E4M3, int LANES>
 cudaError_t read_typed(const KvView& c, const int64_t* slots, int64_t M, void* k, int64_t ldk, void* v, int64_t ldv,
                        cudaStream_t st) {
-    const int64_t b = ceil_div(M * ((k ? 1 : 0) + (v ? 1 : 0)) * c.kv_heads, 256 / LANES);
-    return launch_pdl(kv_read_kernel<T, E4M3, LANES>, dim3((unsigned)(b < kBlocks ? b : kBlocks)), dim3(256), st, c, slots, M,
-                      static_cast<T*>(k), ldk, static_cast<T*>(v), ldv);
+    const int parts = (k ? 1 : 0) + (v ? 1 : 0), per = (int)ceil_div(parts * c.kv_heads, kFlight * (32 / LANES));
+    return launch_pdl(kv_read_kernel<T, E4M3, LANES>, dim3((unsigned)ceil_div(M * per, 8)), dim3(256), st, c, slots, (int)M,
+                      static_cast<T*>(k), ldk, static_cast<T*>(v), ldv, parts, per);
 }
 
-// Lanes for a head of hd values, four each: a power of two that divides a warp.
-#define KV_LANES(fn, T, E, ...)                              \
-    (c.hd > 64   ? fn<T, E, 32>(__VA_ARGS__)                 \
-     : c.hd > 32 ? fn<T, E, 16>(__VA_ARGS__)                 \
-                 : fn<T, E, 8>(__VA_ARGS__))
+// Lanes for a head of hd values, eight each: a power of two that divides a warp.
+#define KV_LANES(fn, T, E, ...)                             \
+    (c.hd > 64   ? fn<T, E, 16>(__VA_ARGS__)                \
+     : c.hd > 32 ? fn<T, E, 8>(__VA_ARGS__)                 \
+                 : fn<T, E, 4>(__VA_ARGS__))
 #define KV_TYPES(fn, ...)                                                                                        \
     (bf16 ? (c.e4m3 ? KV_LANES(fn, __nv_bfloat16, true, __VA_ARGS__) : KV_LANES(fn, __nv_bfloat16, false, __VA_ARGS__)) \
           : (c.e4m3 ? KV_LANES(fn, float, true, __VA_ARGS__) : KV_LANES(fn, float, false, __VA_ARGS__)))

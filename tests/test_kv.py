@@ -147,9 +147,9 @@ def test_workspace_grows_with_the_prefix(b2s):
 def test_binding_refuses_host_tensors_and_shapes(b2s):
     x = torch.zeros(4, 640)
     with pytest.raises(ValueError, match="CUDA"):
-        kv.rope_axes(x, 5, 128, torch.zeros(4, 1, dtype=torch.int32), [64], 1e4, x)
-    with pytest.raises(ValueError, match="rows of"):
-        kv.rope_axes(x, 4, 128, torch.zeros(4, 1, dtype=torch.int32), [64], 1e4, x)
+        kv._rows(x, 640, "x", 0)
+    with pytest.raises(ValueError, match="CUDA"):
+        kv._ints(torch.zeros(4, dtype=torch.int64), torch.int64, (4,), "slots", 0)
     with pytest.raises(ValueError, match="codes"):
         kv.Cache(x, x, x, x)
     k, s = torch.zeros(2, 5, 16, 64, dtype=torch.int8), torch.zeros(2, 5, 16)
