@@ -15,7 +15,7 @@
 //
 // Split: a unit is (sequence, key/value head, eight query rows), its keys are tiles of 32. All units' tiles, laid end to
 // end, are cut into equal ranges, one for each resident block, so that uneven lengths load every SM alike. A block's
-// four warps take the tiles of its range in turn, each through its own ring of three asynchronous copies (no block-wide
+// four warps take the tiles of its range in turn, each through its own ring of asynchronous copies (no block-wide
 // wait between tiles, the ring runs on across units); at a unit's end they are joined through shared memory. A unit cut
 // by a range's border leaves partial results that kv_attention_join_kernel puts together: the order is fixed by the
 // lengths alone, so results do not change from run to run.
@@ -34,13 +34,21 @@ namespace kva {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 32;   // keys per warp step
 constexpr int kRows = 8;    // query rows of a unit
-constexpr int kStages = 3;
-constexpr int kMaxCtas = 320;
-constexpr int kMinTiles = 8;  // a block gets at least this many tiles (two steps of each warp)
+constexpr int kStages = 2;
+constexpr int kPerSm = 3, kMaxCtas = kPerSm * 160;
+constexpr int kMinTiles = 8;     // a block gets at least this many tiles (two steps of each warp)
+constexpr int kWholeTiles = 16;  // units that cannot have more tiles are not cut
 template <int HD>
 constexpr int kStageBytes = 2 * kTile * HD + 2 * kTile * 4 + 128;  // K, V codes, scales, flags
 template <int HD>
 constexpr int kPart = kRows * HD + 2 * kRows;  // floats of a partial result: o, m, l
+// What block c says of the border in front of it, for the join: the pieces of the unit that it cuts, if it is the first one
+// there, and the unit's rows.
+struct Border {
+    int pieces;  // of blocks c - 1, c, ...; 0: nothing to join
+    int slot;    // where block c - 1 left its piece
+    int lo, head0, row0, rows;
+};
 }  // namespace kva
 
 namespace {
@@ -133,11 +141,14 @@ __device__ __forceinline__ Seq seq_of(const KvAttnArgs& a, int b) {
     s.tiles = s.len > kTile ? (s.len + kTile - 1) / kTile : 1;
     return s;
 }
-__device__ __forceinline__ int64_t work_of(const Seq& s) { return (int64_t)s.units * s.tiles; }
+// What ranges are cut in: tiles, or whole units.
+__device__ __forceinline__ int64_t work_of(const Seq& s, const KvAttnArgs& a) {
+    return a.whole_units ? (int64_t)s.units : (int64_t)s.units * s.tiles;
+}
 
 struct Place {
     int b;
-    int64_t off;  // tiles into the sequence's work
+    int64_t off;  // into the sequence's work
 };
 
 // Inclusive sum of v over the block's threads, and the block's total.
@@ -165,6 +176,8 @@ struct Ranges {
     int64_t total;
     int ctas;
     __device__ __forceinline__ int64_t start(int c) const { return total * c / ctas; }
+    // the block that tile x falls to: the last c with start(c) <= x
+    __device__ __forceinline__ int owner(int64_t x) const { return (int)(((x + 1) * ctas + total - 1) / total) - 1; }
 };
 
 // All threads: the total of tiles, how many blocks share them, and the place of block c's first tile (c < ctas).
@@ -172,13 +185,13 @@ __device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, Place& 
     int64_t total = 0, w = 0, incl = 0, sum;
     for (int base = 0; base < a.batch; base += kThreads) {
         const int b = base + threadIdx.x;
-        w = b < a.batch ? work_of(seq_of(a, b)) : 0;
+        w = b < a.batch ? work_of(seq_of(a, b), a) : 0;
         incl = block_scan(w, sh, sum);
         total += sum;
     }
     Ranges r;
     r.total = total;
-    const int64_t want = (total + kMinTiles - 1) / kMinTiles;
+    const int64_t want = a.whole_units ? total : (total + kMinTiles - 1) / kMinTiles;
     r.ctas = (int)(want < gridDim.x ? want : gridDim.x);
     if (c >= r.ctas) return r;
     const int64_t target = r.start(c);
@@ -188,7 +201,7 @@ __device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, Place& 
         int64_t before = 0;
         for (int base = 0; base < a.batch; base += kThreads) {
             const int b = base + threadIdx.x;
-            w = b < a.batch ? work_of(seq_of(a, b)) : 0;
+            w = b < a.batch ? work_of(seq_of(a, b), a) : 0;
             incl = block_scan(w, sh, sum) + before;
             if (target >= incl - w && target < incl) *sh_place = Place{b, target - (incl - w)};
             before += sum;
@@ -204,19 +217,21 @@ struct Walk {
     Seq s;
     int b, u, t0, t1;
     int64_t pos, end;
-    __device__ __forceinline__ void clip() { t1 = (int)min((int64_t)s.tiles, t0 + (end - pos)); }
+    bool whole;
+    __device__ __forceinline__ void clip() { t1 = whole ? s.tiles : (int)min((int64_t)s.tiles, t0 + (end - pos)); }
     __device__ __forceinline__ void begin(const KvAttnArgs& a, const Place& p, int64_t first, int64_t last) {
         b = p.b;
         s = seq_of(a, b);
         pos = first;
         end = last;
-        u = (int)(p.off / s.tiles);
-        t0 = (int)(p.off - (int64_t)u * s.tiles);
+        whole = a.whole_units;
+        u = whole ? (int)p.off : (int)(p.off / s.tiles);
+        t0 = whole ? 0 : (int)(p.off - (int64_t)u * s.tiles);
         clip();
     }
     __device__ __forceinline__ bool done() const { return pos >= end; }
     __device__ __forceinline__ void advance(const KvAttnArgs& a) {
-        pos += t1 - t0;
+        pos += whole ? 1 : t1 - t0;
         if (pos >= end) return;
         if (++u == s.units) {
             u = 0;
@@ -285,7 +300,7 @@ __device__ __forceinline__ void finish(const KvAttnArgs& a, int64_t row, int hea
 
 // ---------------------------------------------------------------- the pass over the keys
 template <int HD, bool E4M3>
-__global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const KvAttnArgs a) {
     constexpr int kChunks = HD / 16;          // 16-byte chunks of a code row
     constexpr int kStage = kStageBytes<HD>;
     constexpr int kWords = HD / 16;           // 4-byte words of a thread's share of a key row (MMA k steps of scores)
@@ -302,7 +317,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
 
     Place place;
     const Ranges rg = find_range(a, blockIdx.x, place, sh_scan, &sh_place);
-    if ((int)blockIdx.x >= rg.ctas) return;
+    Border* border = reinterpret_cast<Border*>(a.part + (int64_t)2 * kMaxCtas * kPart<128>) + blockIdx.x;
+    if ((int)blockIdx.x >= rg.ctas) {
+        if (threadIdx.x == 0) border->pieces = 0;
+        return;
+    }
     const int64_t first = rg.start(blockIdx.x), last = rg.start(blockIdx.x + 1);
     uint8_t* ring = smem + warp * (kStages * kStage);
     const uint32_t ring_u = smem_u32(ring);
@@ -332,25 +351,33 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
     auto issue = [&](int stage) {
         if (have) {
             const uint32_t st = ring_u + stage * kStage;
-            const int k0 = lt * kTile, len = lw.s.len, mask = (1 << a.c.page_shift) - 1;
+            const int k0 = lt * kTile, left = lw.s.len - k0, mask = (1 << a.c.page_shift) - 1;
             const int h = lw.u / lw.s.row_tiles;
             const bool ok_a = page_a >= 0 && page_a < a.c.n_pages, ok_b = page_b >= 0 && page_b < a.c.n_pages;
             if (!(ok_a && ok_b) && lane == 0) atomicOr(&g_device_error, kErrIndex);
-            // cache rows of keys k0 and k0 + 16
+            uint32_t bits = left >= 32 ? 0xffffffffu : (1u << left) - 1u;  // keys there; left > 0 or the sequence is empty
+            if (left <= 0) bits = 0;
+            if (!ok_a) bits &= 0xffff0000u;
+            if (!ok_b) bits &= 0x0000ffffu;
+            // cache rows of keys k0 and (less 16) k0 + 16
             const int64_t ra = (((int64_t)page_a * a.c.kv_heads + h) << a.c.page_shift) + (k0 & mask);
-            const int64_t rb = (((int64_t)page_b * a.c.kv_heads + h) << a.c.page_shift) + ((k0 + 16) & mask);
+            const int64_t rb = (((int64_t)page_b * a.c.kv_heads + h) << a.c.page_shift) + ((k0 + 16) & mask) - 16;
+            constexpr int kRowsAtOnce = 32 / kChunks;
+            const int r0 = lane / kChunks, c = lane % kChunks;
+            const int64_t offa = (ra + r0) * a.c.hd + c * 16, offb = (rb + r0) * a.c.hd + c * 16;
+            const uint32_t mine = c * 16 < a.c.hd ? bits >> r0 : 0u;
 #pragma unroll
-            for (int p = 0; p < kTile * kChunks / 32; ++p) {
-                const int e = p * 32 + lane, r = e / kChunks, c = e % kChunks;
-                const bool on = (r < 16 ? ok_a : ok_b) && k0 + r < len && c * 16 < a.c.hd;
-                const int64_t off = on ? (r < 16 ? ra + r : rb + r - 16) * a.c.hd + c * 16 : 0;
+            for (int p = 0; p < kTile / kRowsAtOnce; ++p) {
+                const int r = p * kRowsAtOnce + r0;
+                const bool on = (mine >> (p * kRowsAtOnce)) & 1;
+                const int64_t off = on ? (p * kRowsAtOnce < 16 ? offa : offb) + p * kRowsAtOnce * a.c.hd : 0;
                 const int f = HD == 128 ? (r & 7) : ((r >> 1) & 3);
                 const uint32_t dst = st + r * HD + ((c ^ f) << 4);
                 cp_async16(dst, a.c.k + off, on);
                 cp_async16(dst + kTile * HD, a.c.v + off, on);
             }
-            const bool on = (lane < 16 ? ok_a : ok_b) && k0 + lane < len;
-            const int64_t row = on ? (lane < 16 ? ra + lane : rb + lane - 16) : 0;
+            const bool on = (bits >> lane) & 1;
+            const int64_t row = on ? (lane < 16 ? ra : rb) + lane : 0;
             cp_async4(st + 2 * kTile * HD + lane * 4, a.c.ks + row, on);
             cp_async4(st + 2 * kTile * HD + kTile * 4 + lane * 4, a.c.vs + row, on);
             if (lane == 0)
@@ -360,50 +387,63 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
         }
         cp_commit();
     };
+    if (threadIdx.x == 0) {
+        Border bd{0, 0, 0, 0, 0, 0};
+        if (cw.t0 > 0) {  // this block's start cuts a unit
+            const int64_t unit = first - cw.t0, before = rg.start(blockIdx.x - 1);
+            if (before <= unit) {  // and no block's before it does
+                const int h = cw.u / cw.s.row_tiles;
+                bd.pieces = rg.owner(unit + cw.s.tiles - 1) - (int)blockIdx.x + 2;
+                bd.slot = before == unit ? 0 : 1;
+                bd.lo = cw.s.lo;
+                bd.head0 = h * a.group;
+                bd.row0 = (cw.u - h * cw.s.row_tiles) * kRows;
+                bd.rows = min(kRows, cw.s.n * a.group - bd.row0);
+            }
+        }
+        *border = bd;
+    }
     fetch();
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) issue(s);
     int it = 0;  // tiles this warp has taken
 
     for (bool head_seg = true; !cw.done(); cw.advance(a), head_seg = false) {
         const int h = cw.u / cw.s.row_tiles, row0 = (cw.u - h * cw.s.row_tiles) * kRows;
         const int rows = min(kRows, cw.s.n * a.group - row0);
-        // ---- the query row of this thread's group, as MMA fragments: k step w holds hd values 4 w' .. 4 w' + 3 of
-        // the thread's contiguous share [t * HD / 4, (t + 1) * HD / 4)
-        uint32_t qh[kWords][2], ql[kWords][2];
-        float rf = 0.0f;  // takes scores back to log2 units
-        int limit = 0;    // keys that the row sees
+        // ---- the query row of this thread's group: its share [t * HD / 4, (t + 1) * HD / 4), as fp32 words
+        uint4 q[kWords];
         {
-            float x[HD / 4];
+            const int r = row0 + min(g, rows - 1), i = a.by_group(r);
+            const int64_t at = (cw.s.lo + (int64_t)i) * a.ldq + (int64_t)(h * a.group + (r - i * a.group)) * a.c.hd + t * (HD / 4);
+            if (a.bf16) {
 #pragma unroll
-            for (int i = 0; i < HD / 4; ++i) x[i] = 0.0f;
-            if (g < rows) {
-                const int r = row0 + g, i = a.by_group(r), head = h * a.group + (r - i * a.group);
-                limit = a.causal ? cw.s.len - cw.s.n + i + 1 : cw.s.len;
-                const int64_t at = (cw.s.lo + (int64_t)i) * a.ldq + (int64_t)head * a.c.hd + t * (HD / 4);
+                for (int j = 0; j < kWords / 2; ++j) {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (t * (HD / 4) + 8 * j < a.c.hd) u = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at)[j];
+                    q[2 * j] = make_uint4(u.x << 16, u.x & 0xffff0000u, u.y << 16, u.y & 0xffff0000u);
+                    q[2 * j + 1] = make_uint4(u.z << 16, u.z & 0xffff0000u, u.w << 16, u.w & 0xffff0000u);
+                }
+            } else {
 #pragma unroll
-                for (int j = 0; j < HD / 4; j += 8) {
-                    if (t * (HD / 4) + j < a.c.hd) {
-                        if (a.bf16) {
-                            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + at + j);
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                x[j + 2 * k] = __uint_as_float(w[k] << 16);
-                                x[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-                            }
-                        } else {
-                            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + j);
-                            const float4 u = p[0], w = p[1];
-                            x[j] = u.x, x[j + 1] = u.y, x[j + 2] = u.z, x[j + 3] = u.w;
-                            x[j + 4] = w.x, x[j + 5] = w.y, x[j + 6] = w.z, x[j + 7] = w.w;
-                        }
-                    }
+                for (int j = 0; j < kWords; ++j) {
+                    q[j] = make_uint4(0, 0, 0, 0);
+                    if (t * (HD / 4) + 4 * j < a.c.hd) q[j] = reinterpret_cast<const uint4*>(static_cast<const float*>(a.q) + at)[j];
                 }
             }
+        }
+        if (head_seg) {  // the rows are on their way while the pages of the first tiles are waited for
+#pragma unroll
+            for (int s = 0; s < kStages - 1; ++s) issue(s);
+        }
+        // ---- as MMA fragments: k step w holds hd values 4 w .. 4 w + 3 of the thread's share
+        uint32_t qh[kWords][2], ql[kWords][2];
+        const int limit = g >= rows ? 0 : a.causal ? cw.s.len - cw.s.n + a.by_group(row0 + g) + 1 : cw.s.len;  // keys the row sees
+        float rf;  // takes scores back to log2 units
+        {
             float big = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 4; ++i) big = fmaxf(big, fabsf(x[i]));
+            for (int w = 0; w < kWords; ++w)
+                big = fmaxf(fmaxf(fmaxf(big, fabsf(__uint_as_float(q[w].x))), fabsf(__uint_as_float(q[w].y))),
+                            fmaxf(fabsf(__uint_as_float(q[w].z)), fabsf(__uint_as_float(q[w].w))));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
             // the row's largest element goes to [2^14, 2^15)
@@ -412,12 +452,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
             rf = __fmul_rn(pow2_biased(254 - up), a.scale_log2e);
 #pragma unroll
             for (int w = 0; w < kWords; ++w) {
-                float y[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] = __fmul_rn(x[4 * w + k], mul);
+                const float y0 = __fmul_rn(__uint_as_float(q[w].x), mul), y1 = __fmul_rn(__uint_as_float(q[w].y), mul);
+                const float y2 = __fmul_rn(__uint_as_float(q[w].z), mul), y3 = __fmul_rn(__uint_as_float(q[w].w), mul);
                 // int8 words unpack to bytes (0, 2) and (1, 3), e4m3 words to (0, 1) and (2, 3)
-                split_h2(y[0], E4M3 ? y[1] : y[2], qh[w][0], ql[w][0]);
-                split_h2(E4M3 ? y[2] : y[1], y[3], qh[w][1], ql[w][1]);
+                split_h2(y0, E4M3 ? y1 : y2, qh[w][0], ql[w][0]);
+                split_h2(E4M3 ? y2 : y1, y3, qh[w][1], ql[w][1]);
             }
         }
         float oacc[kNt][4];
@@ -570,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
             for (int j = 0; j < N; ++j) o[j] = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_m[w][row]);
-#pragma unroll
+#pragma unroll 1
             for (int w = 0; w < kWarps; ++w) {
                 const float mw = sh_m[w][row], f = mw == -INFINITY ? 0.0f : ex2(__fsub_rn(mw, mm));
                 const float* ob = reinterpret_cast<const float*>(smem + (w * kStages + sh_free[w]) * kStage) + row * kOrow +
@@ -600,35 +639,26 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(const KvAttnA
     cp_wait<0>();
 }
 
-// Joins the partial results of every unit that the borders between blocks cut. Block c - 1 looks at border c and acts if
-// it is the first one inside its unit.
+// Joins the partial results of every unit that the borders between blocks cut: block c acts on border c + 1, if it is the
+// first one inside its unit.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(const KvAttnArgs a) {
-    __shared__ int64_t sh_scan[kWarps];
-    __shared__ Place sh_place;
+    constexpr int N = HD / 16;
     griddep_wait();
     griddep_launch();
     const int c = blockIdx.x;
-    Place place;
-    const Ranges rg = find_range(a, c, place, sh_scan, &sh_place);
-    if (c == 0 || c >= rg.ctas) return;
-    const Seq s = seq_of(a, place.b);
-    const int u = (int)(place.off / s.tiles), t = (int)(place.off - (int64_t)u * s.tiles);
-    const int64_t unit = rg.start(c) - t;
-    if (t == 0 || rg.start(c - 1) > unit) return;
-    const int h = u / s.row_tiles, row0 = (u - h * s.row_tiles) * kRows;
-    constexpr int N = HD / 16;
+    const Border bd = reinterpret_cast<const Border*>(a.part + (int64_t)2 * kMaxCtas * kPart<128>)[c + 1];
+    if (bd.pieces == 0) return;
     const int row = threadIdx.x / 16, d = (threadIdx.x % 16) * N;
-    int end = c + 1;
-    while (end < rg.ctas && rg.start(end) < unit + s.tiles) ++end;
-    auto piece = [&](int k) -> const float* {  // pieces of blocks c - 1 .. end - 1
-        return a.part + ((int64_t)k * 2 + (k == c - 1 && rg.start(c - 1) < unit ? 1 : 0)) * kPart<HD>;
-    };
+    if (row >= bd.rows || d >= a.c.hd) return;
+    auto piece = [&](int k) { return a.part + ((int64_t)(c + k) * 2 + (k == 0 ? bd.slot : 0)) * kPart<HD>; };
     float m = -INFINITY, l = 0.0f, o[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = 0.0f;
-    for (int k = c - 1; k < end; ++k) m = fmaxf(m, piece(k)[kRows * HD + row]);
-    for (int k = c - 1; k < end; ++k) {
+#pragma unroll 8
+    for (int k = 0; k < bd.pieces; ++k) m = fmaxf(m, piece(k)[kRows * HD + row]);
+#pragma unroll 4
+    for (int k = 0; k < bd.pieces; ++k) {
         const float* p = piece(k);
         const float mk = p[kRows * HD + row], f = mk == -INFINITY ? 0.0f : ex2(__fsub_rn(mk, m));
         l = __fmaf_rn(p[kRows * HD + kRows + row], f, l);
@@ -641,20 +671,18 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(const KvAtt
             o[j + 3] = __fmaf_rn(v.w, f, o[j + 3]);
         }
     }
-    if (row < min(kRows, s.n * a.group - row0) && d < a.c.hd) {
-        const int r = row0 + row, i = a.by_group(r);
-        finish<N>(a, s.lo + (int64_t)i, h * a.group + (r - i * a.group), d, m, l, o);
-    }
+    const int r = bd.row0 + row, i = a.by_group(r);
+    finish<N>(a, bd.lo + (int64_t)i, bd.head0 + (r - i * a.group), d, m, l, o);
 }
 
 int resident_blocks() {
     static std::atomic<int> cache[128];
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return 2 * 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return kPerSm * 148;
     if (!cache[dev]) {
         int n = 0;
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-        cache[dev] = 2 * n < kMaxCtas ? 2 * n : kMaxCtas;
+        cache[dev] = kPerSm * n < kMaxCtas ? kPerSm * n : kMaxCtas;
     }
     return cache[dev];
 }
@@ -680,13 +708,15 @@ cudaError_t launch_typed(const KvAttnArgs& a, cudaStream_t st) {
     cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kv_attention_kernel<HD, E4M3>), smem);
     if (e != cudaSuccess) return e;
     const int grid = resident_blocks();
-    if ((e = launch_args(kv_attention_kernel<HD, E4M3>, grid, smem, a, st)) != cudaSuccess) return e;
-    return launch_args(kv_attention_join_kernel<HD>, grid, 0, a, st);
+    KvAttnArgs b = a;
+    b.whole_units = (a.max_pages << a.c.page_shift) <= kWholeTiles * kTile;
+    if ((e = launch_args(kv_attention_kernel<HD, E4M3>, grid, smem, b, st)) != cudaSuccess || b.whole_units) return e;
+    return launch_args(kv_attention_join_kernel<HD>, grid - 1, 0, b, st);
 }
 
 }  // namespace
 
-size_t kv_attn_part_bytes() { return sizeof(float) * 2 * kMaxCtas * kPart<128>; }
+size_t kv_attn_part_bytes() { return sizeof(float) * 2 * kMaxCtas * kPart<128> + sizeof(Border) * (kMaxCtas + 1); }
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st) {
     if (a.batch <= 0 || a.M <= 0) return cudaSuccess;

@@ -64,7 +64,8 @@ struct KvAttnArgs {
     bool to_state;           // write `out` instead of o
     AttnState out;           // where it goes, one piece for each split of the keys
     AttnState add;           // joined with the result before it is written; pieces = 0: none
-    float* part;             // split units' partial results (kv_attention.cu)
+    float* part;             // split units' partial results and borders (kv_attention.cu)
+    bool whole_units;        // no unit is split (kv_attention.cu)
 };
 
 // Few rows (kv_attention.cu). to_state writes one piece.
