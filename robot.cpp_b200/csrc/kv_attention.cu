@@ -4,14 +4,18 @@
 // Floor: the cache bytes, (2 hd + 8) per token and key/value head. A decoding step does 4 * group * hd operations on
 // them, so the products only have to keep up with memory.
 //
-// Products: warp-level fp16 MMAs, m16n8k16, fp32 accumulation. 8-bit codes (int8 and e4m3) are exact in fp16, so only
-// the fp32 side of a product is split: a query row, scaled by the power of two that brings its largest element to
-// 2^14, is hi + lo with hi = fp16(x), lo = fp16(x - hi) (relative error 2^-22; elements 2^-38 below the largest one
-// lose bits). The eight rows of a unit are MMA rows 0-7 as hi and 8-15 as lo: one MMA gives both parts and their sum
-// is in one thread. bf16 queries are exact in hi. Probabilities, times the value scale, are split alike.
-//   score(j) = (hi + lo)(q * scale * log2 e) . code(j) * k_scale(j);   p(j) = 2^(score - m);
+//   score(j) = q . code(j) * k_scale(j) * scale * log2 e;   p(j) = 2^(score - m);
 //   o = sum p(j) v_scale(j) code(j) / sum p(j)
-// The value scales are brought into fp16's range by a power of two above the largest one seen (vref).
+// Products: warp-level MMAs with fp32 or int32 accumulation. 8-bit codes (int8 and e4m3) are exact in fp16, so only the
+// fp32 side of a product is split. The eight rows of a unit are MMA rows 0-7 with their larger and 8-15 with their smaller
+// part: one MMA gives both and their sum is in one thread.
+//   e4m3 scores: a query row, scaled by the power of two that brings its largest element to 2^14, is hi + lo with hi =
+//     fp16(x), lo = fp16(x - hi): relative error 2^-22, elements 2^-38 below the largest one lose bits.
+//   int8 scores: the row as integers of 24 bits under its largest element (error 2^-24 of that), in three signed bytes; the
+//     codes go into m16n8k32 integer MMAs as they lie in memory. Unpacking them to fp16 had cost five instructions for four
+//     codes and kept the integer pipe busier than memory.
+//   outputs: the probabilities times the value scale as hi + lo, codes unpacked to fp16. The value scales are brought into
+//     fp16's range by a power of two above the largest one seen (vref).
 //
 // Split: a unit is (sequence, key/value head, eight query rows), its keys are tiles of 32. All units' tiles, laid end to
 // end, are cut into equal ranges, one for each resident block, so that uneven lengths load every SM alike. A block's
@@ -69,6 +73,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// m16n8k32 on signed bytes.
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -101,6 +111,9 @@ __device__ __forceinline__ void unpack4(uint32_t x, uint32_t& p0, uint32_t& p1) 
     }
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
     const int n = on ? 16 : 0;  // 0 bytes: nothing is read, zeros are written
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
@@ -366,6 +379,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
             const int r0 = lane / kChunks, c = lane % kChunks;
             const int64_t offa = (ra + r0) * a.c.hd + c * 16, offb = (rb + r0) * a.c.hd + c * 16;
             const uint32_t mine = c * 16 < a.c.hd ? bits >> r0 : 0u;
+            if (bits == 0xffffffffu && a.c.hd == HD) {  // a whole tile: four pointers and constant steps
+                const uint8_t *ka = a.c.k + offa, *kb = a.c.k + offb, *va = a.c.v + offa, *vb = a.c.v + offb;
+#pragma unroll
+                for (int p = 0; p < kTile / kRowsAtOnce; ++p) {
+                    const int r = p * kRowsAtOnce + r0, f = HD == 128 ? (r & 7) : ((r >> 1) & 3);
+                    const uint32_t dst = st + r * HD + ((c ^ f) << 4);
+                    cp_async16(dst, (p * kRowsAtOnce < 16 ? ka : kb) + p * kRowsAtOnce * HD);
+                    cp_async16(dst + kTile * HD, (p * kRowsAtOnce < 16 ? va : vb) + p * kRowsAtOnce * HD);
+                }
+            } else
 #pragma unroll
             for (int p = 0; p < kTile / kRowsAtOnce; ++p) {
                 const int r = p * kRowsAtOnce + r0;
@@ -434,29 +457,47 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
 #pragma unroll
             for (int s = 0; s < kStages - 1; ++s) issue(s);
         }
-        // ---- as MMA fragments: k step w holds hd values 4 w .. 4 w + 3 of the thread's share
-        uint32_t qh[kWords][2], ql[kWords][2];
+        // ---- as MMA fragments: word w holds hd values 4 w .. 4 w + 3 of the thread's share
+        uint32_t qf[kWords][E4M3 ? 4 : 3];  // e4m3: hi, lo of two pairs; int8: three bytes of each value, largest first
         const int limit = g >= rows ? 0 : a.causal ? cw.s.len - cw.s.n + a.by_group(row0 + g) + 1 : cw.s.len;  // keys the row sees
         float rf;  // takes scores back to log2 units
         {
-            float big = 0.0f;
+            uint32_t bits = 0;  // of the row's largest |q|
 #pragma unroll
             for (int w = 0; w < kWords; ++w)
-                big = fmaxf(fmaxf(fmaxf(big, fabsf(__uint_as_float(q[w].x))), fabsf(__uint_as_float(q[w].y))),
-                            fmaxf(fabsf(__uint_as_float(q[w].z)), fabsf(__uint_as_float(q[w].w))));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // the row's largest element goes to [2^14, 2^15)
-            const int up = min(253, 268 - (__float_as_int(big) >> 23));
-            const float mul = pow2_biased(up);
-            rf = __fmul_rn(pow2_biased(254 - up), a.scale_log2e);
+                bits = max(max(max(bits, q[w].x & 0x7fffffffu), q[w].y & 0x7fffffffu), max(q[w].z & 0x7fffffffu, q[w].w & 0x7fffffffu));
+            bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+            bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
+            float mul;
+            if (E4M3) {  // the row's largest element goes to [2^14, 2^15)
+                const int up = min(253, 268 - (int)(bits >> 23));
+                mul = pow2_biased(up);
+                rf = __fmul_rn(pow2_biased(254 - up), a.scale_log2e);
+            } else {  // to 8355000: three signed bytes hold 8355711
+                const float big = fmaxf(__uint_as_float(bits), 0x1p-100f);
+                mul = __fdiv_rn(8355000.0f, big);
+                rf = __fmul_rn(__fdiv_rn(big, 8355000.0f), a.scale_log2e);
+            }
+            if (bits >= 0x7f800000u) rf = __int_as_float(0x7fc00000);  // an infinity or a NaN makes the row NaN
 #pragma unroll
             for (int w = 0; w < kWords; ++w) {
-                const float y0 = __fmul_rn(__uint_as_float(q[w].x), mul), y1 = __fmul_rn(__uint_as_float(q[w].y), mul);
-                const float y2 = __fmul_rn(__uint_as_float(q[w].z), mul), y3 = __fmul_rn(__uint_as_float(q[w].w), mul);
-                // int8 words unpack to bytes (0, 2) and (1, 3), e4m3 words to (0, 1) and (2, 3)
-                split_h2(y0, E4M3 ? y1 : y2, qh[w][0], ql[w][0]);
-                split_h2(E4M3 ? y2 : y1, y3, qh[w][1], ql[w][1]);
+                const float y[4] = {__fmul_rn(__uint_as_float(q[w].x), mul), __fmul_rn(__uint_as_float(q[w].y), mul),
+                                    __fmul_rn(__uint_as_float(q[w].z), mul), __fmul_rn(__uint_as_float(q[w].w), mul)};
+                if constexpr (E4M3) {  // in the order of unpack4's pairs
+                    split_h2(y[0], y[1], qf[w][0], qf[w][1]);
+                    split_h2(y[2], y[3], qf[w][2], qf[w][3]);
+                } else {
+                    int v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = __float2int_rn(y[k]);
+#pragma unroll
+                    for (int part = 2; part >= 0; --part) {
+                        const uint32_t ab = __byte_perm(v[0], v[1], 0x0040), cd = __byte_perm(v[2], v[3], 0x0040);
+                        qf[w][part] = __byte_perm(ab, cd, 0x5410);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = (v[k] + 128) >> 8;  // what is left above a signed byte
+                    }
+                }
             }
         }
         float oacc[kNt][4];
@@ -481,28 +522,43 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
             float2 vsc[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                float s0, s1;  // products of the row with keys 2 t and 2 t + 1
                 const int r = n * 8 + g;
                 const uint8_t* kr = st + r * HD;
+                uint32_t w[kWords];
 #pragma unroll
                 for (int half = 0; half < kWords / 4; ++half) {
                     const int ch = HD == 128 ? (2 * t + half) ^ (r & 7) : t ^ ((r >> 1) & 3);
                     const uint4 u = *reinterpret_cast<const uint4*>(kr + (ch << 4));
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    w[4 * half] = u.x, w[4 * half + 1] = u.y, w[4 * half + 2] = u.z, w[4 * half + 3] = u.w;
+                }
+                if constexpr (E4M3) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < kWords; ++k) {
                         uint32_t b0, b1;
                         unpack4<E4M3>(w[k], b0, b1);
-                        mma_f16(c, qh[4 * half + k][0], ql[4 * half + k][0], qh[4 * half + k][1], ql[4 * half + k][1], b0, b1);
+                        mma_f16(c, qf[k][0], qf[k][1], qf[k][2], qf[k][3], b0, b1);
                     }
+                    s0 = __fadd_rn(c[0], c[2]);
+                    s1 = __fadd_rn(c[1], c[3]);
+                } else {
+                    int c[4] = {0, 0, 0, 0}, d[4] = {0, 0, 0, 0};  // first and second bytes; third bytes
+#pragma unroll
+                    for (int k = 0; k < kWords; k += 2) {
+                        mma_s8(c, qf[k][0], qf[k][1], qf[k + 1][0], qf[k + 1][1], w[k], w[k + 1]);
+                        mma_s8(d, qf[k][2], 0u, qf[k + 1][2], 0u, w[k], w[k + 1]);
+                    }
+                    s0 = __fmaf_rn((float)(c[0] * 256 + c[2]), 256.0f, (float)d[0]);
+                    s1 = __fmaf_rn((float)(c[1] * 256 + c[3]), 256.0f, (float)d[1]);
                 }
                 const float2 f = *reinterpret_cast<const float2*>(ks + n * 8 + 2 * t);
                 vsc[n] = *reinterpret_cast<const float2*>(vs + n * 8 + 2 * t);
                 const int key = tile * kTile + n * 8 + 2 * t;
                 const bool there = (flags >> (n >> 1)) & 1;
                 const bool see0 = there && key < limit, see1 = there && key + 1 < limit;
-                s[n][0] = see0 ? __fmul_rn(__fmul_rn(__fadd_rn(c[0], c[2]), f.x), rf) : -INFINITY;
-                s[n][1] = see1 ? __fmul_rn(__fmul_rn(__fadd_rn(c[1], c[3]), f.y), rf) : -INFINITY;
+                s[n][0] = see0 ? __fmul_rn(__fmul_rn(s0, f.x), rf) : -INFINITY;
+                s[n][1] = see1 ? __fmul_rn(__fmul_rn(s1, f.y), rf) : -INFINITY;
                 mx = fmaxf(mx, fmaxf(s[n][0], s[n][1]));
                 // a value scale that a row does not see may be anything
                 vsc[n].x = see0 ? vsc[n].x : 0.0f;
