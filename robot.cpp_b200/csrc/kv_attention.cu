@@ -185,12 +185,20 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
     return v + before;
 }
 
+// Whole-number quotient; most are of numbers below 2^32, which divide several times faster.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+// The total in equal shares: the first `more` blocks have one tile more.
 struct Ranges {
-    int64_t total;
-    int ctas;
-    __device__ __forceinline__ int64_t start(int c) const { return total * c / ctas; }
-    // the block that tile x falls to: the last c with start(c) <= x
-    __device__ __forceinline__ int owner(int64_t x) const { return (int)(((x + 1) * ctas + total - 1) / total) - 1; }
+    int64_t total, share;
+    int ctas, more;
+    __device__ __forceinline__ int64_t start(int c) const { return share * c + min(c, more); }
+    // the block that tile x falls to
+    __device__ __forceinline__ int owner(int64_t x) const {
+        const int64_t big = (share + 1) * more;
+        return x < big ? (int)quotient(x, share + 1) : more + (int)quotient(x - big, share);
+    }
 };
 
 // All threads: the total of tiles, how many blocks share them, and the place of block c's first tile (c < ctas).
@@ -207,6 +215,8 @@ __device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, Place& 
     const int64_t want = a.whole_units ? total : (total + kMinTiles - 1) / kMinTiles;
     r.ctas = (int)(want < gridDim.x ? want : gridDim.x);
     if (c >= r.ctas) return r;
+    r.share = quotient(total, r.ctas);
+    r.more = (int)(total - r.share * r.ctas);
     const int64_t target = r.start(c);
     if (a.batch <= kThreads) {
         if (target >= incl - w && target < incl) *sh_place = Place{(int)threadIdx.x, target - (incl - w)};
@@ -238,7 +248,7 @@ struct Walk {
         pos = first;
         end = last;
         whole = a.whole_units;
-        u = whole ? (int)p.off : (int)(p.off / s.tiles);
+        u = whole ? (int)p.off : (int)quotient(p.off, s.tiles);
         t0 = whole ? 0 : (int)(p.off - (int64_t)u * s.tiles);
         clip();
     }
@@ -696,25 +706,27 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
 }
 
 // Joins the partial results of every unit that the borders between blocks cut: block c acts on border c + 1, if it is the
-// first one inside its unit.
+// first one inside its unit. Four groups of threads take every fourth piece, eight in flight; a long unit may have hundreds.
+constexpr int kJoinGroups = 4, kJoinThreads = kThreads * kJoinGroups;
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) kv_attention_join_kernel(const KvAttnArgs a) {
     constexpr int N = HD / 16;
+    __shared__ float sh_m[kJoinGroups][kRows], sh_l[kJoinGroups][kRows];
+    __shared__ __align__(16) float sh_o[kJoinGroups][kRows][HD];
     griddep_wait();
     griddep_launch();
     const int c = blockIdx.x;
     const Border bd = reinterpret_cast<const Border*>(a.part + (int64_t)2 * kMaxCtas * kPart<128>)[c + 1];
     if (bd.pieces == 0) return;
-    const int row = threadIdx.x / 16, d = (threadIdx.x % 16) * N;
-    if (row >= bd.rows || d >= a.c.hd) return;
+    const int group = threadIdx.x / kThreads, row = threadIdx.x % kThreads / 16, d = (threadIdx.x % 16) * N;
     auto piece = [&](int k) { return a.part + ((int64_t)(c + k) * 2 + (k == 0 ? bd.slot : 0)) * kPart<HD>; };
     float m = -INFINITY, l = 0.0f, o[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = 0.0f;
 #pragma unroll 8
-    for (int k = 0; k < bd.pieces; ++k) m = fmaxf(m, piece(k)[kRows * HD + row]);
-#pragma unroll 4
-    for (int k = 0; k < bd.pieces; ++k) {
+    for (int k = group; k < bd.pieces; k += kJoinGroups) m = fmaxf(m, piece(k)[kRows * HD + row]);
+#pragma unroll 8
+    for (int k = group; k < bd.pieces; k += kJoinGroups) {
         const float* p = piece(k);
         const float mk = p[kRows * HD + row], f = mk == -INFINITY ? 0.0f : ex2(__fsub_rn(mk, m));
         l = __fmaf_rn(p[kRows * HD + kRows + row], f, l);
@@ -726,6 +738,26 @@ __global__ void __launch_bounds__(kThreads) kv_attention_join_kernel(const KvAtt
             o[j + 2] = __fmaf_rn(v.z, f, o[j + 2]);
             o[j + 3] = __fmaf_rn(v.w, f, o[j + 3]);
         }
+    }
+    if (d == 0) {
+        sh_m[group][row] = m;
+        sh_l[group][row] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(&sh_o[group][row][d + j]) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+    __syncthreads();
+    if (group != 0 || row >= bd.rows || d >= a.c.hd) return;
+    m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoinGroups; ++k) m = fmaxf(m, sh_m[k][row]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoinGroups; ++k) {
+        const float f = sh_m[k][row] == -INFINITY ? 0.0f : ex2(__fsub_rn(sh_m[k][row], m));
+        l = __fmaf_rn(sh_l[k][row], f, l);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = __fmaf_rn(sh_o[k][row][d + j], f, o[j]);
     }
     const int r = bd.row0 + row, i = a.by_group(r);
     finish<N>(a, bd.lo + (int64_t)i, bd.head0 + (r - i * a.group), d, m, l, o);
@@ -744,10 +776,10 @@ int resident_blocks() {
 }
 
 template <typename K>
-cudaError_t launch_args(K kernel, int grid, size_t smem, const KvAttnArgs& a, cudaStream_t st) {
+cudaError_t launch_args(K kernel, int grid, int block, size_t smem, const KvAttnArgs& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -766,8 +798,8 @@ cudaError_t launch_typed(const KvAttnArgs& a, cudaStream_t st) {
     const int grid = resident_blocks();
     KvAttnArgs b = a;
     b.whole_units = (a.max_pages << a.c.page_shift) <= kWholeTiles * kTile;
-    if ((e = launch_args(kv_attention_kernel<HD, E4M3>, grid, smem, b, st)) != cudaSuccess || b.whole_units) return e;
-    return launch_args(kv_attention_join_kernel<HD>, grid - 1, 0, b, st);
+    if ((e = launch_args(kv_attention_kernel<HD, E4M3>, grid, kThreads, smem, b, st)) != cudaSuccess || b.whole_units) return e;
+    return launch_args(kv_attention_join_kernel<HD>, grid - 1, kJoinThreads, 0, b, st);
 }
 
 }  // namespace
