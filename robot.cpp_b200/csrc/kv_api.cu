@@ -79,28 +79,47 @@ int cache_view(const b2s_kv_cache* c, b2s::KvView* v, const char* op) {
 // kernel, which reads them once per 128.
 constexpr int kFewRows = 64;
 struct Plan {
-    bool few, many, pair;
+    bool few, many, pair;  // pair: blocks of 256 rows
     int min_rows, splits;
 };
-Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
-    Plan p{true, false, false, 0, 1};
-    if (max_q * group <= kFewRows) return p;
-    p.many = true;
-    p.few = M != batch * max_q;  // equal: every sequence has max_q rows
-    p.min_rows = p.few ? kFewRows : 0;
-    // Less than a wave of blocks: cut the keys, so that waves x (tiles of 128 keys + about four tiles' worth of
-    // starting and ending a block) is least.
-    p.pair = bf16 && max_q * group > 128;
-    const int block = p.pair ? 256 : 128;
+// The tensor-core kernel's part of a plan for M tokens of up to max_q a sequence over `keys` keys.
+void plan_blocks(Plan* p, int64_t M, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
+    p->many = true;
+    p->pair = bf16 && max_q * group > 128;
+    // Less than a wave of blocks: cut the keys, so that waves x (tiles of 128 keys + about four tiles' worth of starting and
+    // ending a block) is least.
+    const int block = p->pair ? 256 : 128;
     const int64_t units = std::max<int64_t>(1, M * group / block) * kv_heads, tiles = (keys + 127) / 128;
     int64_t best = 0;
+    p->splits = 1;
     for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles) && units < 148; ++s) {
         const int64_t cost = (units * s + 147) / 148 * ((tiles + s - 1) / s + 4) + (s > 1 ? 3 : 0);
         if (s == 1 || cost < best) {
             best = cost;
-            p.splits = s;
+            p->splits = s;
         }
     }
+}
+Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
+    Plan p{true, false, false, 0, 1};
+    if (max_q * group <= kFewRows) return p;
+    plan_blocks(&p, M, max_q, group, kv_heads, keys, bf16);
+    p.few = M != batch * max_q;  // equal: every sequence has max_q rows
+    p.min_rows = p.few ? kFewRows : 0;
+    return p;
+}
+
+// A shared prefix goes through the tensor-core kernel, once for all rows, unless few rows make it cheaper to let every
+// sequence read it with its own tokens (from L2): up to kPrefixSteps steps of 32 keys and eight rows. One pass then takes the
+// place of three: 16 rows on 545 shared tokens (1440 steps) took 26 us in passes of their own.
+constexpr int64_t kPrefixSteps = 8192;
+Plan plan_prefix(const Plan& own, int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t prefix_len, bool bf16) {
+    Plan p{false, false, false, 0, 1};
+    if (prefix_len == 0) return p;
+    if (!own.many && batch * kv_heads * ((max_q * group + 7) / 8) * ((prefix_len + 31) / 32) <= kPrefixSteps)
+        p.few = true;
+    else
+        plan_blocks(&p, M, M, group, kv_heads, prefix_len, bf16);
     return p;
 }
 
@@ -113,7 +132,7 @@ struct AttnWs {
     size_t part, total;
     StateWs own, prefix;
 };
-AttnWs attn_ws(const Plan& own, const Plan& pre, int64_t M, int heads, int hd, int64_t prefix_len) {
+AttnWs attn_ws(const Plan& own, const Plan& pre, int64_t M, int heads, int hd) {
     AttnWs w;
     w.part = 0;
     w.total = a256(b2s::kv_attn_part_bytes());
@@ -127,8 +146,8 @@ AttnWs attn_ws(const Plan& own, const Plan& pre, int64_t M, int heads, int hd, i
         w.total = s.o + a256(rows * hd * sizeof(float));
         return s;
     };
-    w.own = take(own.many && (own.splits > 1 || prefix_len > 0) ? own.splits : 0);
-    w.prefix = take(prefix_len > 0 ? (pre.many ? pre.splits : 1) : 0);
+    w.own = take(own.many && (own.splits > 1 || pre.many) ? own.splits : 0);
+    w.prefix = take(pre.many ? pre.splits : 0);
     return w;
 }
 
@@ -140,8 +159,8 @@ int check_shapes(const b2s::KvView& v, const b2s_kv_batch* b, int64_t M, int n_h
         return fail(B2S_ERR_INVALID_ARG, "%s: %d query heads on %d key/value heads", op, n_heads, v.kv_heads);
     if (b->batch > kMaxBatch) return fail(B2S_ERR_UNSUPPORTED, "%s: %d sequences, at most %d", op, b->batch, kMaxBatch);
     const int64_t most = kMaxInt - 1024;
-    if (M > most / n_heads || b->max_pages > (most >> v.page_shift) || prefix_len > most)
-        return fail(B2S_ERR_UNSUPPORTED, "%s: rows x heads, tokens of a sequence and prefix_len have to be below 2^31", op);
+    if (M > most / n_heads || prefix_len > most || b->max_pages > ((most - prefix_len) >> v.page_shift))
+        return fail(B2S_ERR_UNSUPPORTED, "%s: rows x heads and prefix_len + tokens of a sequence have to be below 2^31", op);
     return B2S_OK;
 }
 
@@ -164,10 +183,10 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     }
     if (prefix_len > 0 && !prefix_pages) return fail(B2S_ERR_INVALID_ARG, "%s: prefix_pages is NULL", op);
     const int group = n_heads / v.kv_heads;
-    const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift,
-                               type == B2S_TYPE_BF16);
-    const Plan pre = plan_rows(M, 1, M, group, v.kv_heads, prefix_len, type == B2S_TYPE_BF16);
-    const AttnWs w = attn_ws(own, pre, M, n_heads, v.hd, prefix_len);
+    const bool bf16 = type == B2S_TYPE_BF16;
+    const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift, bf16);
+    const Plan pre = plan_prefix(own, M, batch->batch, batch->max_q, group, v.kv_heads, prefix_len, bf16);
+    const AttnWs w = attn_ws(own, pre, M, n_heads, v.hd);
     if (!workspace || workspace_bytes < w.total)
         return fail(B2S_ERR_WORKSPACE, "%s needs %zu workspace bytes, got %zu", op, w.total, workspace ? workspace_bytes : 0);
     if (!aligned(workspace, 256)) return fail(B2S_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", op);
@@ -188,25 +207,23 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     while ((1u << a.group_shift) < (uint32_t)group) ++a.group_shift;  // n / group as a multiplication, for n < 2^31
     a.group_mul = (uint32_t)((((uint64_t)1 << 32) * ((1u << a.group_shift) - (uint32_t)group)) / (uint32_t)group + 1);
     a.scale_log2e = scale * 1.4426950408889634f;
-    a.bf16 = type == B2S_TYPE_BF16;
+    a.bf16 = bf16;
     a.part = reinterpret_cast<float*>(ws + w.part);
     a.q_start = batch->q_start;
     auto state = [&](const StateWs& s) {
         return b2s::AttnState{reinterpret_cast<float*>(ws + s.m), reinterpret_cast<float*>(ws + s.l),
                               reinterpret_cast<float*>(ws + s.o), s.pieces};
     };
-    if (prefix_len > 0) {  // the batch's rows as one sequence over the prefix
+    if (pre.many) {  // the batch's rows as one sequence over the prefix
         b2s::KvAttnArgs p = a;
         p.batch = 1;
         p.q_stride = batch->batch;
         p.kv_const = prefix_len;
         p.pages = prefix_pages;
         p.max_pages = (prefix_len + cache->page_size - 1) / cache->page_size;
-        p.max_rows = (int)kMaxInt;
         p.to_state = true;
         p.out = state(w.prefix);
-        rc = launched(pre.many ? b2s::launch_kv_attention_tc(p, pre.pair, pre.splits, st) : b2s::launch_kv_attention(p, st), op);
-        if (rc) return rc;
+        if ((rc = launched(b2s::launch_kv_attention_tc(p, pre.pair, pre.splits, st), op))) return rc;
         a.add = p.out;
     }
     a.batch = batch->batch;
@@ -226,6 +243,10 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     }
     if (!own.few) return B2S_OK;
     a.max_rows = own.many ? kFewRows : (int)kMaxInt;
+    if (pre.few) {
+        a.prefix_pages = prefix_pages;
+        a.prefix_len = (int)prefix_len;
+    }
     return launched(b2s::launch_kv_attention(a, st), op);
 }
 
@@ -320,10 +341,11 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache* cache, const b2s_kv_b
     if (check_shapes(v, batch, M, n_heads, prefix_len, "attention_kv_workspace_size")) return 0;
     const int group = n_heads / v.kv_heads;
     size_t most = 0;
-    for (int bf16 = 0; bf16 < 2; ++bf16)  // either type
-        most = std::max(most, attn_ws(plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift, bf16),
-                                      plan_rows(M, 1, M, group, v.kv_heads, prefix_len, bf16), M, n_heads, v.hd, prefix_len)
-                                  .total);
+    for (int bf16 = 0; bf16 < 2; ++bf16) {  // either type
+        const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift, bf16);
+        const Plan pre = plan_prefix(own, M, batch->batch, batch->max_q, group, v.kv_heads, prefix_len, bf16);
+        most = std::max(most, attn_ws(own, pre, M, n_heads, v.hd).total);
+    }
     return most;
 }
 

@@ -41,9 +41,9 @@ constexpr int kRows = 8;    // query rows of a unit
 constexpr int kStages = 2;
 constexpr int kPerSm = 3, kMaxCtas = kPerSm * 160;
 constexpr int kMinTiles = 8;     // a block gets at least this many tiles (two steps of each warp)
-constexpr int kWholeTiles = 16;  // units that cannot have more tiles are not cut
+constexpr int kWholeTiles = 24;  // units that cannot have more tiles are not cut
 template <int HD>
-constexpr int kStageBytes = 2 * kTile * HD + 2 * kTile * 4 + 128;  // K, V codes, scales, flags
+constexpr int kStageBytes = 2 * kTile * HD + 2 * kTile * 4 + 128;  // K, V codes, scales, which keys are there
 template <int HD>
 constexpr int kPart = kRows * HD + 2 * kRows;  // floats of a partial result: o, m, l
 // What block c says of the border in front of it, for the join: the pieces of the unit that it cuts, if it is the first one
@@ -129,6 +129,7 @@ __device__ __forceinline__ void cp_wait() {
 }
 
 // ---------------------------------------------------------------- units
+// A sequence's keys as the kernel counts them: a shared prefix padded to whole tiles, then its own.
 struct Seq {
     int lo, n, len;    // first query row, query rows, keys
     int row_tiles, units, tiles;
@@ -147,7 +148,7 @@ __device__ __forceinline__ Seq seq_of(const KvAttnArgs& a, int b) {
         len = len < 0 ? 0 : cap;
     }
     if (bad) atomicOr(&g_device_error, kErrIndex);
-    s.len = (int)len;
+    s.len = a.prefix_pad + (int)len;
     const int rows = s.n * a.group;
     s.row_tiles = rows > a.min_rows && rows <= a.max_rows ? (rows + kRows - 1) / kRows : 0;
     s.units = s.row_tiles * a.c.kv_heads;
@@ -287,17 +288,6 @@ __device__ __forceinline__ void finish(const KvAttnArgs& a, int64_t row, int hea
         }
         m = mn;
     }
-    if (a.to_state) {
-        const int64_t i = row * a.heads + head;
-        if (d == 0) {
-            a.out.m[i] = m;
-            a.out.l[i] = l;
-        }
-        float* p = a.out.o + i * a.c.hd + d;
-#pragma unroll
-        for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-        return;
-    }
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = l == 0.0f ? 0.0f : __fmul_rn(o[j], inv);
@@ -322,7 +312,7 @@ __device__ __forceinline__ void finish(const KvAttnArgs& a, int64_t row, int hea
 }
 
 // ---------------------------------------------------------------- the pass over the keys
-template <int HD, bool E4M3>
+template <int HD, bool E4M3, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const KvAttnArgs a) {
     constexpr int kChunks = HD / 16;          // 16-byte chunks of a code row
     constexpr int kStage = kStageBytes<HD>;
@@ -334,6 +324,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
     __shared__ int64_t sh_scan[kWarps];
     __shared__ Place sh_place;
     __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
+    __shared__ Walk sh_load[kWarps], sh_walk[2];
+    __shared__ int sh_free[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     griddep_wait();
     griddep_launch();
@@ -349,37 +341,57 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
     uint8_t* ring = smem + warp * (kStages * kStage);
     const uint32_t ring_u = smem_u32(ring);
 
-    Walk cw;
-    cw.begin(a, place, first, last);
+    // The way through the range is kept in shared memory: for each warp's loader, which runs ahead, and (two slots in turn)
+    // for the block. Registers hold what a tile needs.
+    if (lane == 0) {
+        Walk w;
+        w.begin(a, place, first, last);
+        sh_load[warp] = w;
+        if (warp == 0) sh_walk[0] = w;
+    }
+    __syncthreads();
 
     // ---- loader: the warp's tiles in order, one ahead with the page numbers
-    Walk lw = cw;
-    int lt = lw.t0 + warp;
+    int lt, lt_end, l_len, l_head, l_seq;
+    auto take_load = [&]() {
+        const Walk& w = sh_load[warp];
+        lt = w.t0 + warp;
+        lt_end = w.t1;
+        l_len = w.s.len;
+        l_head = w.u / w.s.row_tiles;
+        l_seq = w.b;
+    };
+    take_load();
     int page_a = 0, page_b = 0;
     bool have = true;
     auto fetch = [&]() {  // the next tile of this warp, and the pages of its two halves
-        while (lt >= lw.t1) {
-            lw.advance(a);
-            if (lw.done()) {
+        while (lt >= lt_end) {
+            __syncwarp();
+            if (lane == 0) sh_load[warp].advance(a);
+            __syncwarp();
+            if (sh_load[warp].done()) {
                 have = false;
                 return;
             }
-            lt = lw.t0 + warp;
+            take_load();
         }
         const int k0 = lt * kTile;
-        const int32_t* pg = a.pages + (int64_t)lw.b * a.ld_pages;
-        page_a = k0 < lw.s.len ? pg[k0 >> a.c.page_shift] : 0;
-        page_b = k0 + 16 < lw.s.len ? pg[(k0 + 16) >> a.c.page_shift] : 0;
+        const bool own = !PREFIX || k0 >= a.prefix_pad;
+        const int32_t* pg = own ? a.pages + (int64_t)l_seq * a.ld_pages : a.prefix_pages;
+        const int k = PREFIX && own ? k0 - a.prefix_pad : k0;
+        const int end = !PREFIX ? l_len : own ? l_len - a.prefix_pad : a.prefix_len;
+        page_a = k < end ? pg[k >> a.c.page_shift] : 0;
+        page_b = k + 16 < end ? pg[(k + 16) >> a.c.page_shift] : 0;
     };
     auto issue = [&](int stage) {
         if (have) {
             const uint32_t st = ring_u + stage * kStage;
-            const int k0 = lt * kTile, left = lw.s.len - k0, mask = (1 << a.c.page_shift) - 1;
-            const int h = lw.u / lw.s.row_tiles;
+            const int at = lt * kTile, k0 = PREFIX && at >= a.prefix_pad ? at - a.prefix_pad : at;  // in the own keys or the prefix
+            const int left = (!PREFIX || at >= a.prefix_pad ? l_len : a.prefix_len) - at, mask = (1 << a.c.page_shift) - 1;
+            const int h = l_head;
             const bool ok_a = page_a >= 0 && page_a < a.c.n_pages, ok_b = page_b >= 0 && page_b < a.c.n_pages;
             if (!(ok_a && ok_b) && lane == 0) atomicOr(&g_device_error, kErrIndex);
-            uint32_t bits = left >= 32 ? 0xffffffffu : (1u << left) - 1u;  // keys there; left > 0 or the sequence is empty
-            if (left <= 0) bits = 0;
+            uint32_t bits = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;  // keys there
             if (!ok_a) bits &= 0xffff0000u;
             if (!ok_b) bits &= 0x0000ffffu;
             // cache rows of keys k0 and (less 16) k0 + 16
@@ -413,14 +425,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
             const int64_t row = on ? (lane < 16 ? ra : rb) + lane : 0;
             cp_async4(st + 2 * kTile * HD + lane * 4, a.c.ks + row, on);
             cp_async4(st + 2 * kTile * HD + kTile * 4 + lane * 4, a.c.vs + row, on);
-            if (lane == 0)
-                *reinterpret_cast<int*>(ring + stage * kStage + 2 * kTile * HD + 2 * kTile * 4) = (ok_a ? 1 : 0) | (ok_b ? 2 : 0);
+            if (lane == 0) *reinterpret_cast<uint32_t*>(ring + stage * kStage + 2 * kTile * HD + 2 * kTile * 4) = bits;
             lt += kWarps;
             fetch();
         }
         cp_commit();
     };
     if (threadIdx.x == 0) {
+        const Walk& cw = sh_walk[0];
         Border bd{0, 0, 0, 0, 0, 0};
         if (cw.t0 > 0) {  // this block's start cuts a unit
             const int64_t unit = first - cw.t0, before = rg.start(blockIdx.x - 1);
@@ -439,9 +451,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
     fetch();
     int it = 0;  // tiles this warp has taken
 
-    for (bool head_seg = true; !cw.done(); cw.advance(a), head_seg = false) {
+    for (int seg = 0; !sh_walk[seg & 1].done(); ++seg) {
+        const bool head_seg = seg == 0;
+        const Walk& cw = sh_walk[seg & 1];
         const int h = cw.u / cw.s.row_tiles, row0 = (cw.u - h * cw.s.row_tiles) * kRows;
-        const int rows = min(kRows, cw.s.n * a.group - row0);
+        const int rows = min(kRows, cw.s.n * a.group - row0), seg_end = cw.t1;
         // ---- the query row of this thread's group: its share [t * HD / 4, (t + 1) * HD / 4), as fp32 words
         uint4 q[kWords];
         {
@@ -469,7 +483,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
         }
         // ---- as MMA fragments: word w holds hd values 4 w .. 4 w + 3 of the thread's share
         uint32_t qf[kWords][E4M3 ? 4 : 3];  // e4m3: hi, lo of two pairs; int8: three bytes of each value, largest first
-        const int limit = g >= rows ? 0 : a.causal ? cw.s.len - cw.s.n + a.by_group(row0 + g) + 1 : cw.s.len;  // keys the row sees
+        // keys that the row sees: the whole prefix and its own
+        const int limit = g >= rows ? 0 : a.causal ? max(PREFIX ? a.prefix_pad : 0, cw.s.len - cw.s.n + a.by_group(row0 + g) + 1) : cw.s.len;
         float rf;  // takes scores back to log2 units
         {
             uint32_t bits = 0;  // of the row's largest |q|
@@ -518,14 +533,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
         float m = -INFINITY, l = 0.0f;
         int vref = 15;  // biased exponent above every value scale so far
 
-        for (int tile = cw.t0 + warp; tile < cw.t1; tile += kWarps, ++it) {
+        for (int tile = cw.t0 + warp; tile < seg_end; tile += kWarps, ++it) {
             cp_wait<kStages - 2>();
             __syncwarp();
             issue((it + kStages - 1) % kStages);
             const uint8_t* st = ring + (it % kStages) * kStage;
             const float* ks = reinterpret_cast<const float*>(st + 2 * kTile * HD);
             const float* vs = ks + kTile;
-            const int flags = *reinterpret_cast<const int*>(vs + kTile);
+            const uint32_t there = *reinterpret_cast<const uint32_t*>(vs + kTile);
             // ---- scores of 32 keys: thread (g, t) gets keys 8 n + 2 t, 8 n + 2 t + 1 of row g
             float s[4][2];
             float mx = -INFINITY, vmax = 0.0f;
@@ -565,8 +580,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
                 const float2 f = *reinterpret_cast<const float2*>(ks + n * 8 + 2 * t);
                 vsc[n] = *reinterpret_cast<const float2*>(vs + n * 8 + 2 * t);
                 const int key = tile * kTile + n * 8 + 2 * t;
-                const bool there = (flags >> (n >> 1)) & 1;
-                const bool see0 = there && key < limit, see1 = there && key + 1 < limit;
+                const uint32_t here = there >> (n * 8 + 2 * t);
+                const bool see0 = (here & 1) && key < limit, see1 = (here & 2) && key + 1 < limit;
                 s[n][0] = see0 ? __fmul_rn(__fmul_rn(s0, f.x), rf) : -INFINITY;
                 s[n][1] = see1 ? __fmul_rn(__fmul_rn(s1, f.y), rf) : -INFINITY;
                 mx = fmaxf(mx, fmaxf(s[n][0], s[n][1]));
@@ -664,8 +679,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
                     *reinterpret_cast<float4*>(ob + half * kNt + n) = x;
                 }
         }
-        __shared__ int sh_free[kWarps];
         if (lane == 0) sh_free[warp] = free_stage;
+        if (threadIdx.x == 0) {  // the next segment; everybody reads it behind the last barrier of this one
+            Walk w = cw;
+            w.advance(a);
+            sh_walk[(seg + 1) & 1] = w;
+        }
         __syncthreads();
         {
             constexpr int N = HD / 16;
@@ -790,16 +809,22 @@ cudaError_t launch_args(K kernel, int grid, int block, size_t smem, const KvAttn
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <int HD, bool E4M3>
+template <int HD, bool E4M3, bool PREFIX>
 cudaError_t launch_typed(const KvAttnArgs& a, cudaStream_t st) {
     const size_t smem = (size_t)kWarps * kStages * kStageBytes<HD>;
-    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kv_attention_kernel<HD, E4M3>), smem);
+    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kv_attention_kernel<HD, E4M3, PREFIX>), smem);
     if (e != cudaSuccess) return e;
     const int grid = resident_blocks();
     KvAttnArgs b = a;
-    b.whole_units = (a.max_pages << a.c.page_shift) <= kWholeTiles * kTile;
-    if ((e = launch_args(kv_attention_kernel<HD, E4M3>, grid, kThreads, smem, b, st)) != cudaSuccess || b.whole_units) return e;
+    b.prefix_pad = (int)round_up(a.prefix_len, kTile);
+    b.whole_units = b.prefix_pad + (a.max_pages << a.c.page_shift) <= kWholeTiles * kTile;
+    if ((e = launch_args(kv_attention_kernel<HD, E4M3, PREFIX>, grid, kThreads, smem, b, st)) != cudaSuccess || b.whole_units)
+        return e;
     return launch_args(kv_attention_join_kernel<HD>, grid - 1, kJoinThreads, 0, b, st);
+}
+template <int HD, bool E4M3>
+cudaError_t launch_prefix(const KvAttnArgs& a, cudaStream_t st) {
+    return a.prefix_len > 0 ? launch_typed<HD, E4M3, true>(a, st) : launch_typed<HD, E4M3, false>(a, st);
 }
 
 }  // namespace
@@ -808,8 +833,8 @@ size_t kv_attn_part_bytes() { return sizeof(float) * 2 * kMaxCtas * kPart<128> +
 
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st) {
     if (a.batch <= 0 || a.M <= 0) return cudaSuccess;
-    if (a.c.hd > 64) return a.c.e4m3 ? launch_typed<128, true>(a, st) : launch_typed<128, false>(a, st);
-    return a.c.e4m3 ? launch_typed<64, true>(a, st) : launch_typed<64, false>(a, st);
+    if (a.c.hd > 64) return a.c.e4m3 ? launch_prefix<128, true>(a, st) : launch_prefix<128, false>(a, st);
+    return a.c.e4m3 ? launch_prefix<64, true>(a, st) : launch_prefix<64, false>(a, st);
 }
 
 }  // namespace b2s

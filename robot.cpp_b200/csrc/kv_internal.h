@@ -61,14 +61,17 @@ struct KvAttnArgs {
     float scale_log2e;       // scale * log2(e): scores are in log2 units
     int causal;
     bool bf16;
-    bool to_state;           // write `out` instead of o
+    bool to_state;           // write `out` instead of o (kv_attention_tc.cu alone)
     AttnState out;           // where it goes, one piece for each split of the keys
     AttnState add;           // joined with the result before it is written; pieces = 0: none
     float* part;             // split units' partial results and borders (kv_attention.cu)
-    bool whole_units;        // no unit is split (kv_attention.cu)
+    // kv_attention.cu alone
+    bool whole_units;               // no unit is split
+    const int32_t* prefix_pages;    // tokens in front of every sequence, read with its own
+    int prefix_len, prefix_pad;     // prefix_pad: in whole tiles
 };
 
-// Few rows (kv_attention.cu). to_state writes one piece.
+// Few rows (kv_attention.cu).
 size_t kv_attn_part_bytes();
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st);
 
