@@ -8,16 +8,21 @@
 //
 // A block takes rows (tokens x the heads of a group) of one sequence and key/value head and walks its keys in tiles of 128.
 // Four warps bring codes from the pages, unpack them and store fp16 tiles in the 128-byte swizzled layout that serves K as a
-// K-major and V as an MN-major operand. Two groups of eight warps do the softmax from tensor memory, two threads a row, and
-// write P over S; one thread of each issues the group's MMAs. While one group's products run the other is at its
-// exponentials. Sixteen warps because one warp a scheduler needs 570 clocks for 32 keys' exponentials, four need 280 each
-// (measured alone; the special-function unit's own limit is 256). The groups are
+// K-major and V as an MN-major operand. Two groups of eight warps do the softmax from tensor memory, one thread for each row
+// and half of a tile's keys, and write P over S. The groups are
 //   PAIR: two blocks of 128 rows that share every unpacked tile (bf16, where unpacking would weigh as much as the products);
 //   else: the even and the odd key tiles of the same 128 rows, each with its own reference, sum and outputs, joined at the
 //         end (fp32, whose two-part queries leave no room for more rows; and bf16 calls that have no more).
+// A group's two halves are streams of their own: 128 threads, 64 columns of S and P, one thread that issues the stream's MMAs.
+// A stream's chain (scores, exponentials, outputs, the next scores over its P) has four others' work beside it: with one
+// chain a group the tensor cores and the exponentials waited for each other (a pair of tiles took 7500 clocks, of which the
+// products are 2048 and the exponentials 2048). Sixteen warps also because one warp a scheduler needs 570 clocks for 32 keys'
+// exponentials and four need 280 each (measured alone; the special-function unit's own limit is 256).
 // The reference of the exponentials is a whole number that moves only when probabilities grow past 2^8: sums, outputs and
-// the tile's probabilities are then multiplied by a power of two, which is exact. So scores are read once and no maximum is
-// formed: 32 probabilities whose sum is at most 2^8 are each at most that, and only a larger sum asks for their maximum.
+// probabilities are then multiplied by a power of two, which is exact. So scores are read once and no maximum is formed: 32
+// probabilities whose sum is at most 2^8 are each at most that, and only a larger sum asks for their maximum. A row's
+// outputs have one reference; its two streams commit their products to it in turn, and whoever finds the other's reference
+// changed brings its own probabilities, or the outputs, under the larger one.
 //
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
 // MMAs are issued, those in flight are waited for, and tensor memory is freed.
@@ -33,7 +38,8 @@ namespace b2s {
 namespace kvt {
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kSoftWarps = 16, kConvWarps = 4, kThreads = 32 * (kSoftWarps + kConvWarps);
-constexpr int kTmemCols = 512, kOcol = 256;  // S/P of the two warpgroups at 0 and 128, O at 256 and 384
+constexpr int kHalf = kKeys / 2;
+constexpr int kTmemCols = 512, kOcol = 256;  // S/P of the four streams at 0, 64, 128, 192, O of the two groups at 256 and 384
 constexpr int kBlock = kKeys * 128;          // bytes of 128 rows x 64 fp16 values
 struct Misc {
     float ks[4][kKeys];        // key scales of four tiles in flight, times the factor that takes scores to log2 units
@@ -41,9 +47,10 @@ struct Misc {
     float vn[4][kKeys];        // value scales over the power of two above the largest finite one of their 32 keys
     int vexp[4][kConvWarps];   // that one's biased exponent, 1..252
     uint32_t there[4][kConvWarps];  // keys that exist
-    float m[2][2][kRows], l[2][2][kRows], back[2][kRows];  // [group][half of the row's keys][row]
-    int wmin[2][4];  // fewest keys that a row of a group's four row warps sees
-    uint64_t qfull, kfull[2], kfree[2], vfull[2], vfree[2], sfull[2], pvd[2], scfull[4], turn, drain[2];
+    float om[2][kRows];        // [group][row] reference of the row's outputs: of the exponentials,
+    int ov[2][kRows];          // and of the value scales
+    float l[2][2][kRows];      // [group][half of the row's keys][row]
+    uint64_t qfull, kfull[2], kfree[2], vfull[2], vfree[2], sfull[4], pvd[4], mpost[4], scfull[4], drain[4];
     int64_t scan[kThreads / 32];
     int64_t found[2];
     float big[kSoftWarps];
@@ -96,6 +103,10 @@ __device__ __forceinline__ void unpack4(uint32_t w, uint32_t& p0, uint32_t& p1) 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
     const int n = on ? 16 : 0;  // 0 bytes: nothing is read, zeros are written
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t at, uint4 x) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 
 // V as an MN-major operand with 128-byte swizzle: 64 values of hd are 128 bytes, 8 keys make an atom (stride 1024), the
@@ -307,15 +318,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ms->kfull[i], 32 * kConvWarps);
             mbar_init(&ms->vfull[i], 32 * kConvWarps);
-            mbar_init(&ms->kfree[i], PAIR ? 2 : 1);
-            mbar_init(&ms->vfree[i], PAIR ? 2 : 1);
+            mbar_init(&ms->kfree[i], PAIR ? 4 : 2);
+            mbar_init(&ms->vfree[i], PAIR ? 4 : 2);
+        }
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&ms->sfull[i], 1);
             mbar_init(&ms->pvd[i], 1);
+            mbar_init(&ms->mpost[i], kRows);
             mbar_init(&ms->drain[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&ms->scfull[i], 32 * kConvWarps);
         mbar_init(&ms->qfull, 32 * kSoftWarps);
-        mbar_init(&ms->turn, 2 * kRows);
         ms->abort = 0;
         fence_mbar_init();
     }
@@ -411,16 +424,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 vsc = __ldg(a.c.vs + row);
             }
         };
-        const uint32_t at = (cw * 32 + rsub) * 128 + (((2 * cc) ^ rsub) << 4);
-        auto store = [&](uint8_t* tile, int i, uint4 r) {
+        const uint32_t at = (cw * 32 + rsub) * 128 + (((2 * cc) ^ rsub) << 4), k_at = smem_u32(sK) + at, v_at = smem_u32(sV) + at;
+        auto store = [&](uint32_t tile, int i, uint4 r) {
             uint32_t w[8];
             unpack4<E4M3>(r.x, w[0], w[1]);
             unpack4<E4M3>(r.y, w[2], w[3]);
             unpack4<E4M3>(r.z, w[4], w[5]);
             unpack4<E4M3>(r.w, w[6], w[7]);
             const int off = (i % kBlk) * kBlock + (i / kBlk) * 1024;
-            *reinterpret_cast<uint4*>(tile + at + off) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(tile + (at ^ 16) + off) = make_uint4(w[4], w[5], w[6], w[7]);
+            st_shared16(tile + off, make_uint4(w[0], w[1], w[2], w[3]));
+            st_shared16((tile ^ 16) + off, make_uint4(w[4], w[5], w[6], w[7]));
         };
         // Order of the tiles: K0, K1, V0, K2, V1, ...: the next tile's scores do not wait for this one's V. Each is asked for
         // when the one before it of its kind has been stored.
@@ -437,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             const int st = j & 1, sc = j & 3;
             if (j >= 2) wait(ms, &ms->kfree[st], (uint32_t)((j >> 1) - 1) & 1u);
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) store(sK + st * kTileBytes, i, kr[i]);
+            for (int i = 0; i < kChunks; ++i) store(k_at + st * kTileBytes, i, kr[i]);
             fence_proxy_async_smem();
             mbar_arrive(&ms->kfull[st]);
             if (j == 0) {
@@ -465,9 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             if (j >= 0) {
                 if (j >= 2) wait(ms, &ms->vfree[j & 1], (uint32_t)((j >> 1) - 1) & 1u);
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll 2
+#pragma unroll
                 for (int i = 0; i < kChunks; ++i)
-                    store(sV + (j & 1) * kTileBytes, i, *reinterpret_cast<const uint4*>(mine + i * (32 * kConvWarps * 16)));
+                    store(v_at + (j & 1) * kTileBytes, i, *reinterpret_cast<const uint4*>(mine + i * (32 * kConvWarps * 16)));
                 fence_proxy_async_smem();
                 mbar_arrive(&ms->vfull[j & 1]);
             }
@@ -548,115 +561,80 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         }
         const int wg = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, r = quad * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-        const uint32_t sbuf = lane_addr + wg * kKeys, obuf = lane_addr + kOcol + wg * kRows + half * (HDP / 2);
+        const int st = 2 * wg + half;  // stream
+        const uint32_t sbuf = lane_addr + st * kHalf, obuf = lane_addr + kOcol + wg * kRows;
         const int rb = row0 + (PAIR ? wg * kRows : 0) + r;  // row of the sequence
         const bool mine = rb < row0 + rows;
         const int tok = a.by_group(rb);
         // a row that is not there never masks (its results are dropped)
         const int limit = !mine ? 0x7fffffff : a.causal ? sq.len - sq.n + tok + 1 : sq.len;
-        {
-            const int w = __reduce_min_sync(0xffffffffu, limit);
-            if (half == 0 && lane == 0) ms->wmin[wg][quad] = w;
-        }
-        auto group_sync = [&]() {
-            tc_fence_before();
-            asm volatile("bar.sync %0, 256;" ::"r"(2 + wg) : "memory");
-            tc_fence_after();
-        };
-        auto group_any = [&](bool x) {  // whether any thread of the group has x; a barrier
-            uint32_t y = x;
-            tc_fence_before();
-            asm volatile(
-                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbar.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                : "+r"(y)
-                : "r"(2 + wg)
-                : "memory");
-            tc_fence_after();
-            return y != 0;
-        };
-        group_sync();
-        const int wmin = min(min(ms->wmin[wg][0], ms->wmin[wg][1]), min(ms->wmin[wg][2], ms->wmin[wg][3]));
+        const int wmin = __reduce_min_sync(0xffffffffu, limit);
         const int n = PAIR ? nt : (nt + 1 - wg) / 2;
-        float m = -INFINITY, l = 0.0f;  // the two threads of a row have the same m, and l of their keys
+        float m = -INFINITY, l = 0.0f;  // reference and sum of this thread's keys
         int vref = 8;
-        // ---- this group's MMAs, issued by its first warp
-        const bool leader = (warp & 7) == 0;
-        const uint32_t q0 = smem_u32(sQ) + (PAIR ? wg * kTileBytes : 0), s0 = tmem + wg * kKeys, o0 = tmem + kOcol + wg * kRows;
+        // ---- this stream's MMAs, issued by one of its warps: another scheduler's for each stream
+        const bool leader = quad == st;
+        const uint32_t q0 = smem_u32(sQ) + (PAIR ? wg * kTileBytes : 0), s0 = tmem + st * kHalf, o0 = tmem + kOcol + wg * kRows;
         volatile int* ab = &ms->abort;
         auto issue_scores = [&](int i) {
             const int j = PAIR ? i : 2 * i + wg;
             wait(ms, &ms->kfull[j & 1], (uint32_t)(j >> 1) & 1u);
             if (__any_sync(0xffffffffu, *ab)) return;
             tc_fence_after();
-            const uint32_t kt = smem_u32(sK) + (j & 1) * kTileBytes;
+            const uint32_t kt = smem_u32(sK) + (j & 1) * kTileBytes + half * (kHalf * 128);
             const uint64_t qd = umma_desc_k_sw128(q0), kd = umma_desc_k_sw128(kt);
 #pragma unroll
             for (int k = 0; k < PARTS * (HDP / 16); ++k) {  // the small part first: fewer roundings of large sums
                 const int part = PARTS - 1 - k / (HDP / 16), s = k % (HDP / 16);
                 const uint32_t off = ((s >> 2) * kBlock + (s & 3) * 32) >> 4;
-                mma_ss(s0, qd + (part * kTileBytes >> 4) + off, kd + off, idesc_f16(kKeys, false), k > 0 ? 1u : 0u);
+                mma_ss(s0, qd + (part * kTileBytes >> 4) + off, kd + off, idesc_f16(kHalf, false), k > 0 ? 1u : 0u);
             }
-            commit_elected(&ms->sfull[wg]);
+            commit_elected(&ms->sfull[st]);
             commit_elected(&ms->kfree[j & 1]);
         };
         auto issue_outputs = [&](int i) {
             const int j = PAIR ? i : 2 * i + wg;
             wait(ms, &ms->vfull[j & 1], (uint32_t)(j >> 1) & 1u);
+            // behind the other stream's product, so that the order of the sums is always the same
+            if (i + half > 0) wait(ms, &ms->pvd[st ^ 1], (uint32_t)(half ? i : i - 1) & 1u);
             if (__any_sync(0xffffffffu, *ab)) return;
             tc_fence_after();
-            const uint32_t vt = smem_u32(sV) + (j & 1) * kTileBytes;
+            const uint32_t vt = smem_u32(sV) + (j & 1) * kTileBytes + half * (kHalf * 128);
             const uint64_t vd = desc_mn_sw128(vt);
 #pragma unroll
-            for (int k = 0; k < PARTS * (kKeys / 16); ++k) {  // P of 32 keys: 16 columns of the large parts, 16 of the small ones
-                const int part = PARTS - 1 - k / (kKeys / 16), s = k % (kKeys / 16);
+            for (int k = 0; k < PARTS * (kHalf / 16); ++k) {  // P of 32 keys: 16 columns of the large parts, 16 of the small ones
+                const int part = PARTS - 1 - k / (kHalf / 16), s = k % (kHalf / 16);
                 mma_ts(o0, s0 + (s >> 1) * 32 + part * 16 + (s & 1) * 8, vd + (s * 2048 >> 4), idesc_f16(HDP, true),
-                       k > 0 ? 1u : i > 0 ? 1u : 0u);
+                       k > 0 ? 1u : i + half > 0 ? 1u : 0u);
             }
-            commit_elected(&ms->pvd[wg]);
+            commit_elected(&ms->pvd[st]);
             commit_elected(&ms->vfree[j & 1]);
         };
-        if (leader) {
-            wait(ms, &ms->qfull, 0);
-            if (PAIR && wg == 1 && n > 0) wait(ms, &ms->turn, 0);  // half a tile behind: one computes while the other's products run
-        }
+        if (leader) wait(ms, &ms->qfull, 0);
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
             const int j = PAIR ? i : 2 * i + wg, sc = j & 3;
             if (leader) {
-                if (i > 0) wait(ms, &ms->pvd[wg], (uint32_t)(i - 1) & 1u);  // these scores overwrite P
+                if (i > 0) wait(ms, &ms->pvd[st], (uint32_t)(i - 1) & 1u);  // these scores overwrite P
                 issue_scores(i);
             }
             __syncwarp();
             wait(ms, &ms->scfull[sc], (uint32_t)(j >> 2) & 1u);
-            const uint4 there = *reinterpret_cast<const uint4*>(ms->there[sc]);
-            const int key0 = (t0 + j) * kKeys;
-            const bool edge = (there.x & there.y & there.z & there.w) != 0xffffffffu || key0 + kKeys > wmin;
+            const uint2 there = *reinterpret_cast<const uint2*>(&ms->there[sc][2 * half]);
+            const int key0 = (t0 + j) * kKeys + half * kHalf;
+            const bool masked = __any_sync(0xffffffffu, (there.x & there.y) != 0xffffffffu || key0 + kHalf > wmin);
             // keys of 32 that the row sees
             auto see_of = [&](int c) {
                 const int left = limit - (key0 + 32 * c);
-                return ms->there[sc][c] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
+                return ms->there[sc][2 * half + c] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
             };
-            wait(ms, &ms->sfull[wg], (uint32_t)i & 1u);
-            // Every choice between barriers is the group's, by a barrier of its own: it is one even if a wait ran out.
-            const bool masked = group_any(edge);
-            // From here on the outputs of the last tile are complete.
-            auto scale_outputs = [&](float f) {  // this thread's half of the columns
-                if (i == 0) return;
-#pragma unroll 1
-                for (int c = 0; c < HDP / 2; c += 16) {
-                    uint32_t x[16];
-                    tmem_ld_x16(obuf + c, x);
-                    wait_ld(x);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__fmul_rn(__uint_as_float(x[k]), f));
-                    tmem_st_x16(obuf + c, x);
-                }
-            };
-            auto scale_probabilities = [&](int c0, int c1, float f) {  // chunks c0 .. c1 - 1 of the tile
+            wait(ms, &ms->sfull[st], (uint32_t)i & 1u);
+            tc_fence_after();
+            auto scale_probabilities = [&](int chunks, float f) {  // the half tile's first chunks of 32 keys
                 tc_wait_st();
                 const __half2 f2h = __float2half2_rn(f);
 #pragma unroll 1
-                for (int c = 32 * c0; c < 32 * c1; c += PARTS == 1 ? 32 : 16) {
+                for (int c = 0; c < 32 * chunks; c += PARTS == 1 ? 32 : 16) {
                     uint32_t x[16];
                     tmem_ld_x16(sbuf + c, x);
                     wait_ld(x);
@@ -673,18 +651,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 const float by = __fsub_rn(from, to);
                 return by >= -126.0f ? pow2_biased(127 + (int)by) : 0.0f;
             };
-            // The power of two that value scales are kept under; e is the same for a row's two threads.
-            auto widen = [&](int e) {
-                const bool up = e >= vref;
-                if (!__any_sync(0xffffffffu, up)) return;
-                float f = 1.0f;
-                if (up) {
-                    const int nref = min(e + 2, 255);
-                    f = nref - vref > 126 ? 0.0f : pow2_biased(127 - (nref - vref));
-                    vref = nref;
-                }
-                scale_outputs(f);
-            };
             auto part = [&](F2 w, uint32_t& hi, uint32_t& lo) {
                 float u, v;
                 unf2(w, u, v);
@@ -696,16 +662,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 }
             };
             if (!masked) {
-                const int4 ve = *reinterpret_cast<const int4*>(ms->vexp[sc]);
-                widen(max(max(ve.x, ve.y), max(ve.z, ve.w)));
+                const int e = max(ms->vexp[sc][2 * half], ms->vexp[sc][2 * half + 1]);
+                if (e >= vref) vref = min(e + 2, 255);
                 // P of 32 keys over their scores: p = 2^(s - m + shift) times the value scales, which are over 2^(exponent + 1)
                 // of their 32 keys (one far below the reference counts as 2^-60); their sum is taken back by 2^-shift
-                const float m0 = m;
 #pragma unroll 1
-                for (int c = 2 * half; c < 2 * half + 2; ++c) {
-                    const float4* ksp = reinterpret_cast<const float4*>(&ms->ks[sc][32 * c]);
-                    const float4* vnp = reinterpret_cast<const float4*>(&ms->vn[sc][32 * c]);
-                    const int shift = max(-60, ms->vexp[sc][c] + 7 - vref);
+                for (int c = 0; c < 2; ++c) {
+                    const float4* ksp = reinterpret_cast<const float4*>(&ms->ks[sc][half * kHalf + 32 * c]);
+                    const float4* vnp = reinterpret_cast<const float4*>(&ms->vn[sc][half * kHalf + 32 * c]);
+                    const int shift = max(-60, ms->vexp[sc][2 * half + c] + 7 - vref);
                     const float most = pow2_biased(127 + 8 + shift);
                     uint32_t x[32];
                     float sum;
@@ -746,7 +711,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                             mx = max3(mx, __fmul_rn(__uint_as_float(x[4 * k]), f.x), __fmul_rn(__uint_as_float(x[4 * k + 1]), f.y));
                             mx = max3(mx, __fmul_rn(__uint_as_float(x[4 * k + 2]), f.z), __fmul_rn(__uint_as_float(x[4 * k + 3]), f.w));
                         }
-                        // m follows here for this thread's keys, and for the row behind the barrier
                         float f = 1.0f;
                         if (mx > __fadd_rn(m, 8.0f)) {
                             const float mn = ceilf(mx);
@@ -754,59 +718,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                             l = __fmul_rn(l, f);
                             m = mn;
                         }
-                        if (c & 1) scale_probabilities(c - 1, c, f);
+                        if (c > 0) scale_probabilities(1, f);
                     }
                     l = __fmaf_rn(sum, pow2_biased(127 - shift), l);
                 }
-                ms->m[wg][half][r] = m;
-                tc_wait_st();
-                const bool moved = group_any(m != m0);
-                if (moved) {
-                    const float mn = fmaxf(m, ms->m[wg][half ^ 1][r]), f = down(m, mn);
-                    if (__any_sync(0xffffffffu, m != mn)) {
-                        scale_probabilities(2 * half, 2 * half + 2, f);
-                        l = __fmul_rn(l, f);
-                    }
-                    scale_outputs(down(m0, mn));
-                    m = mn;
-                    tc_wait_st();
-                    group_sync();
-                }
             } else {  // a key or value scale that the row does not see may be anything
                 float mx = -INFINITY, vmx = 0.0f;
+                const float* kp = &ms->ks[sc][half * kHalf];
+                const float* vp = &ms->vs[sc][half * kHalf];
 #pragma unroll 1
-                for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     const uint32_t see = see_of(c >> 1) >> (16 * (c & 1));
                     uint32_t x[16];
                     tmem_ld_x16(sbuf + 16 * c, x);
                     wait_ld(x);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float u = __fmul_rn(__uint_as_float(x[k]), ms->ks[sc][16 * c + k]);
+                        const float u = __fmul_rn(__uint_as_float(x[k]), kp[16 * c + k]);
                         if ((see >> k) & 1) {
                             mx = fmaxf(mx, u);
-                            vmx = fmaxf(vmx, fabsf(ms->vs[sc][16 * c + k]));
+                            vmx = fmaxf(vmx, fabsf(vp[16 * c + k]));
                         }
                     }
                 }
-                ms->m[wg][half][r] = mx;
-                ms->l[wg][half][r] = vmx;
-                group_sync();
-                mx = fmaxf(mx, ms->m[wg][half ^ 1][r]);
-                vmx = fmaxf(vmx, ms->l[wg][half ^ 1][r]);
-                widen(__float_as_int(vmx) >> 23);
-                const bool up = mx > __fadd_rn(m, 8.0f);
-                if (__any_sync(0xffffffffu, up)) {
-                    const float mn = up ? ceilf(mx) : m, f = up ? down(m, mn) : 1.0f;
-                    l = __fmul_rn(l, f);
+                const int e = __float_as_int(vmx) >> 23;
+                if (e >= vref) vref = min(e + 2, 255);
+                if (mx > __fadd_rn(m, 8.0f)) {
+                    const float mn = ceilf(mx);
+                    l = __fmul_rn(l, down(m, mn));
                     m = mn;
-                    tc_wait_st();
-                    scale_outputs(f);
                 }
                 const float mu = m == -INFINITY ? 0.0f : -m, vmul = pow2_biased(260 - vref);
                 uint32_t keep[8];
 #pragma unroll 1
-                for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     const uint32_t see = see_of(c >> 1) >> (16 * (c & 1));
                     uint32_t x[16];
                     tmem_ld_x16(sbuf + 16 * c, x);
@@ -820,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                         for (int q = 0; q < 2; ++q) {
                             const int key = 16 * c + 2 * k + q;
                             const bool on = (see >> (2 * k + q)) & 1;
-                            p[q] = on ? ex2(__fmaf_rn(__uint_as_float(x[2 * k + q]), ms->ks[sc][key], mu)) : 0.0f;
-                            w[q] = on ? __fmul_rn(p[q], __fmul_rn(ms->vs[sc][key], vmul)) : 0.0f;
+                            p[q] = on ? ex2(__fmaf_rn(__uint_as_float(x[2 * k + q]), kp[key], mu)) : 0.0f;
+                            w[q] = on ? __fmul_rn(p[q], __fmul_rn(vp[key], vmul)) : 0.0f;
                         }
                         sum = __fadd_rn(sum, __fadd_rn(p[0], p[1]));
                         part(f2(w[0], w[1]), hi[k], lo[k]);
@@ -841,42 +786,80 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                     }
                     l = __fadd_rn(l, sum);
                 }
-                tc_wait_st();
-                group_sync();
             }
-            if (PAIR && wg == 0 && i == 0) mbar_arrive(&ms->turn);
+            // ---- one reference for the row's outputs: the other stream has left the one that its last half tile went in with
+            if (i + half > 0) wait(ms, &ms->mpost[st ^ 1], (uint32_t)(half ? i : i - 1) & 1u);
+            const float mo = i + half > 0 ? ms->om[wg][r] : -INFINITY;
+            const int vo = i + half > 0 ? ms->ov[wg][r] : 8;
+            if (__any_sync(0xffffffffu, m != mo || vref != vo)) {
+                const float mn = fmaxf(m, mo);
+                const int vn = max(vref, vo);
+                const float fm = m == mn ? 1.0f : down(m, mn);
+                const float fp = __fmul_rn(fm, vn - vref > 126 ? 0.0f : pow2_biased(127 - (vn - vref)));
+                const float fo = __fmul_rn(mo == mn ? 1.0f : down(mo, mn), vn - vo > 126 ? 0.0f : pow2_biased(127 - (vn - vo)));
+                l = __fmul_rn(l, fm);
+                if (__any_sync(0xffffffffu, fp != 1.0f)) scale_probabilities(2, fp);
+                if (i + half > 0 && __any_sync(0xffffffffu, fo != 1.0f)) {
+                    wait(ms, &ms->pvd[st ^ 1], (uint32_t)(half ? i : i - 1) & 1u);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HDP; c += 16) {
+                        uint32_t x[16];
+                        tmem_ld_x16(obuf + c, x);
+                        wait_ld(x);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__fmul_rn(__uint_as_float(x[k]), fo));
+                        tmem_st_x16(obuf + c, x);
+                    }
+                }
+                m = mn;
+                vref = vn;
+            }
+            ms->om[wg][r] = m;
+            ms->ov[wg][r] = vref;
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&ms->mpost[st]);
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + st) : "memory");
+            tc_fence_after();
             if (leader) issue_outputs(i);
             __syncwarp();
         }
-        if (n > 0) {
-            wait(ms, &ms->pvd[wg], (uint32_t)(n - 1) & 1u);
+        if (n > 0) {  // the second stream's last product is the group's last
+            wait(ms, &ms->pvd[st | 1], (uint32_t)(n - 1) & 1u);
             tc_fence_after();
         }
         if (leader) {  // also after a wait that ran out: what was issued finishes before tensor memory is freed
-            commit_elected(&ms->drain[wg]);
-            mbar_wait(&ms->drain[wg], 0, 2u);
+            commit_elected(&ms->drain[st]);
+            mbar_wait(&ms->drain[st], 0, 2u);
         }
         __syncwarp();
         // ---- results: half of the columns of its row for each thread, a quarter where both groups have the same rows
-        ms->m[wg][half][r] = m;
-        ms->l[wg][half][r] = l;
-        if (half == 0) ms->back[wg][r] = pow2_biased(vref - 6);
-        if (PAIR) {
-            group_sync();
+        if (n == 0) {
+            ms->om[wg][r] = -INFINITY;
+            ms->ov[wg][r] = 8;
         } else {
-            tc_fence_before();
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-            tc_fence_after();
+            wait(ms, &ms->mpost[st | 1], (uint32_t)(n - 1) & 1u);
+            const float mf = ms->om[wg][r];  // the last reference
+            if (m != mf) l = m == -INFINITY ? 0.0f : __fmul_rn(l, ex2(__fsub_rn(m, mf)));
         }
-        float f0 = ms->back[wg][r], f1 = 0.0f;
+        ms->l[wg][half][r] = l;
+        tc_fence_before();
+        if (PAIR)
+            asm volatile("bar.sync %0, 256;" ::"r"(6 + wg) : "memory");
+        else
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+        tc_fence_after();
+        float f0 = pow2_biased(ms->ov[wg][r] - 6), f1 = 0.0f;
+        m = ms->om[wg][r];
         l = __fadd_rn(ms->l[wg][0][r], ms->l[wg][1][r]);
         if (!PAIR) {
-            const float ma = ms->m[0][0][r], mb = ms->m[1][0][r];
+            const float ma = ms->om[0][r], mb = ms->om[1][r];
             m = fmaxf(ma, mb);
             const float fa = ma == -INFINITY ? 0.0f : ex2(__fsub_rn(ma, m)), fb = mb == -INFINITY ? 0.0f : ex2(__fsub_rn(mb, m));
             l = __fmaf_rn(__fadd_rn(ms->l[0][0][r], ms->l[0][1][r]), fa, __fmul_rn(__fadd_rn(ms->l[1][0][r], ms->l[1][1][r]), fb));
-            f0 = __fmul_rn(ms->back[0][r], fa);
-            f1 = __fmul_rn(ms->back[1][r], fb);
+            f0 = __fmul_rn(pow2_biased(ms->ov[0][r] - 6), fa);
+            f1 = __fmul_rn(pow2_biased(ms->ov[1][r] - 6), fb);
         }
         const int c0 = PAIR ? half * (HDP / 2) : (2 * wg + half) * (HDP / 4), c1 = c0 + (PAIR ? HDP / 2 : HDP / 4);
         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
