@@ -41,6 +41,9 @@ constexpr int kSoftWarps = 16, kConvWarps = 4, kThreads = 32 * (kSoftWarps + kCo
 constexpr int kHalf = kKeys / 2;
 constexpr int kTmemCols = 512, kOcol = 256;  // S/P of the four streams at 0, 64, 128, 192, O of the two groups at 256 and 384
 constexpr int kBlock = kKeys * 128;          // bytes of 128 rows x 64 fp16 values
+struct Rows {
+    int lo, n, len, rows;  // first query row, query rows, keys, (token, head of group) rows that this pass takes
+};
 struct Misc {
     float ks[4][kKeys];        // key scales of four tiles in flight, times the factor that takes scores to log2 units
     float vs[4][kKeys];        // value scales
@@ -53,6 +56,7 @@ struct Misc {
     uint64_t qfull, kfull[2], kfree[2], vfull[2], vfree[2], sfull[4], pvd[4], mpost[4], scfull[4], drain[4];
     int64_t scan[kThreads / 32];
     int64_t found[2];
+    Rows seq;                  // that sequence
     float big[kSoftWarps];
     uint32_t tmem;
     int abort;
@@ -211,9 +215,6 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
     return r;
 }
 
-struct Rows {
-    int lo, n, len, rows;  // first query row, query rows, keys, (token, head of group) rows that this pass takes
-};
 __device__ __forceinline__ Rows rows_of(const KvAttnArgs& a, int b) {
     Rows s;
     const int lo = a.q_start[b * a.q_stride], hi = a.q_start[(b + 1) * a.q_stride];
@@ -272,13 +273,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
 
     // ---- which sequence, row block, head and share of the keys: later row blocks, which see more keys, go first
     const int h = blockIdx.x % a.c.kv_heads;
-    const int64_t rest = blockIdx.x / a.c.kv_heads;
-    const int split = (int)(rest / units);
-    int unit = (int)(rest - (int64_t)split * units);
+    const int rest = blockIdx.x / a.c.kv_heads, split = rest / units;
+    int unit = rest - split * units;
     {
+        Rows seq;
         auto scan = [&](int base, int64_t& w, int64_t& sum) {  // blocks of the sequences up to this thread's, and of all
             const int b = base + tid;
-            w = b < a.batch ? (rows_of(a, b).rows + kBlkRows - 1) / kBlkRows : 0;
+            if (b < a.batch) seq = rows_of(a, b);
+            w = b < a.batch ? (seq.rows + kBlkRows - 1) / kBlkRows : 0;
             int64_t v = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -308,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             if (unit >= incl - w && unit < incl) {
                 ms->found[0] = base + tid;
                 ms->found[1] = unit - (incl - w);
+                ms->seq = seq;
             }
             if (base == 0 || unit >= before) break;
             incl = scan(base - kThreads, w, sum);
@@ -341,12 +344,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, ms->tmem, 0);
     const int b = (int)ms->found[0], row0 = (int)ms->found[1] * kBlkRows;
-    const Rows sq = rows_of(a, b);
+    const Rows sq = ms->seq;
     const int rows = min(kBlkRows, sq.rows - row0);
     // keys that the last row sees
     const int most = a.causal ? min(sq.len, max(0, sq.len - sq.n + a.by_group(row0 + rows - 1) + 1)) : sq.len;
     const int all_tiles = (most + kKeys - 1) / kKeys;
-    const int t0 = (int)((int64_t)all_tiles * split / splits), nt = (int)((int64_t)all_tiles * (split + 1) / splits) - t0;
+    const int t0 = (unsigned)(all_tiles * split) / (unsigned)splits, nt = (unsigned)(all_tiles * (split + 1)) / (unsigned)splits - t0;
 
     // The power of two that all query rows share: the largest finite element goes to [2^14, 2^15).
     auto common_up = [&]() {
@@ -728,7 +731,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 const float* vp = &ms->vs[sc][half * kHalf];
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    const uint32_t see = see_of(c >> 1) >> (16 * (c & 1));
+                    const uint32_t see = (see_of(c >> 1) >> (16 * (c & 1))) & 0xffffu;
+                    if (!__any_sync(0xffffffffu, see)) continue;  // mostly so on a causal diagonal: 32 rows are few tokens
                     uint32_t x[16];
                     tmem_ld_x16(sbuf + 16 * c, x);
                     wait_ld(x);
@@ -752,24 +756,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 uint32_t keep[8];
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    const uint32_t see = see_of(c >> 1) >> (16 * (c & 1));
-                    uint32_t x[16];
-                    tmem_ld_x16(sbuf + 16 * c, x);
+                    const uint32_t see = (see_of(c >> 1) >> (16 * (c & 1))) & 0xffffu;
                     float sum = 0.0f;
                     uint32_t hi[8], lo[8];
-                    wait_ld(x);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        float p[2], w[2];
+                    for (int k = 0; k < 8; ++k) hi[k] = lo[k] = 0;
+                    if (__any_sync(0xffffffffu, see)) {
+                        uint32_t x[16];
+                        tmem_ld_x16(sbuf + 16 * c, x);
+                        wait_ld(x);
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const int key = 16 * c + 2 * k + q;
-                            const bool on = (see >> (2 * k + q)) & 1;
-                            p[q] = on ? ex2(__fmaf_rn(__uint_as_float(x[2 * k + q]), kp[key], mu)) : 0.0f;
-                            w[q] = on ? __fmul_rn(p[q], __fmul_rn(vp[key], vmul)) : 0.0f;
+                        for (int k = 0; k < 8; ++k) {
+                            float p[2], w[2];
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const int key = 16 * c + 2 * k + q;
+                                const bool on = (see >> (2 * k + q)) & 1;
+                                p[q] = on ? ex2(__fmaf_rn(__uint_as_float(x[2 * k + q]), kp[key], mu)) : 0.0f;
+                                w[q] = on ? __fmul_rn(p[q], __fmul_rn(vp[key], vmul)) : 0.0f;
+                            }
+                            sum = __fadd_rn(sum, __fadd_rn(p[0], p[1]));
+                            part(f2(w[0], w[1]), hi[k], lo[k]);
                         }
-                        sum = __fadd_rn(sum, __fadd_rn(p[0], p[1]));
-                        part(f2(w[0], w[1]), hi[k], lo[k]);
                     }
                     const uint32_t to = sbuf + 32 * (c >> 1) + 8 * (c & 1);
                     // the chunk's second 16 scores lie where its small parts go: they are kept until those are read
@@ -845,10 +853,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         }
         ms->l[wg][half][r] = l;
         tc_fence_before();
-        if (PAIR)
-            asm volatile("bar.sync %0, 256;" ::"r"(6 + wg) : "memory");
-        else
-            asm volatile("bar.sync 1, 512;" ::: "memory");
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // every product has been made: Q and K are not read any more
         tc_fence_after();
         float f0 = pow2_biased(ms->ov[wg][r] - 6), f1 = 0.0f;
         m = ms->om[wg][r];
@@ -863,13 +868,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         }
         const int c0 = PAIR ? half * (HDP / 2) : (2 * wg + half) * (HDP / 4), c1 = c0 + (PAIR ? HDP / 2 : HDP / 4);
         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-        const int64_t grow = sq.lo + (int64_t)tok;
-        const int head = h * a.group + (rb - tok * a.group);
-        const int64_t si = ((int64_t)split * a.M + grow) * a.heads + head;
         if (a.to_state && mine && c0 == 0) {
+            const int64_t si = ((int64_t)split * a.M + sq.lo + tok) * a.heads + h * a.group + (rb - tok * a.group);
             a.out.m[si] = m;
             a.out.l[si] = l;
         }
+        // Rows go through shared memory, over Q (fp32 pieces of bf16 rows also over K), so that a warp writes whole ones
+        const int lg = PARTS == 2 || a.to_state ? 2 : 1;  // bytes of an element, as a shift
+        uint8_t* to = sQ + (((PAIR ? wg * kRows : 0) + r) * HDP << lg);
         const uint32_t oa = lane_addr + kOcol + (PAIR ? wg * kRows : 0);
 #pragma unroll 1
         for (int d = c0; d < c1; d += 16) {
@@ -880,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             if (!PAIR && nt > 1) tmem_ld_x16(oa + kRows + d, y);
             wait_ld(x);
             if (!PAIR) wait_ld(y);
-            if (!mine || d >= a.c.hd) continue;
+            if (d >= a.c.hd) continue;
             float o[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -895,30 +901,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                     o[k + 2] = z;
                 }
             }
-            if (a.to_state) {
-                float4* p = reinterpret_cast<float4*>(a.out.o + si * a.c.hd + d);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) p[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                continue;
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = l == 0.0f ? 0.0f : __fmul_rn(o[k], inv);
-            const int64_t at = grow * a.ldo + (int64_t)head * a.c.hd + d;
-            if (PARTS == 1) {
-                uint4* p = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + at);
+            for (int k = 0; k < 16; ++k) o[k] = a.to_state ? o[k] : l == 0.0f ? 0.0f : __fmul_rn(o[k], inv);
+            if (lg == 1) {
                 uint32_t w[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const __nv_bfloat162 z = __floats2bfloat162_rn(o[2 * k], o[2 * k + 1]);
                     w[k] = *reinterpret_cast<const uint32_t*>(&z);
                 }
-                p[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                p[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            } else {
-                float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.o) + at);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) p[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                for (int k = 0; k < 2; ++k)
+                    *reinterpret_cast<uint4*>(to + (((d >> 3) + k) ^ (r & 7)) * 16) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<float4*>(to + (((d >> 2) + k) ^ (r & 7)) * 16) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
             }
+        }
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+        const int sh = (HDP == 128 ? 3 : 2) + lg, per = 1 << sh;  // 16-byte pieces of a row
+#pragma unroll 4
+        for (int i = tid; i < rows * per; i += 32 * kSoftWarps) {
+            const int rr = i >> sh, c = i & (per - 1), t = a.by_group(row0 + rr);
+            const uint4 u = *reinterpret_cast<const uint4*>(sQ + (rr * HDP << lg) + (c ^ (rr & 7)) * 16);
+            if (c << (4 - lg) >= a.c.hd) continue;
+            const int64_t grow = sq.lo + (int64_t)t;
+            const int head = h * a.group + (row0 + rr - t * a.group);
+            uint8_t* p = a.to_state ? reinterpret_cast<uint8_t*>(a.out.o + (((int64_t)split * a.M + grow) * a.heads + head) * a.c.hd)
+                                    : static_cast<uint8_t*>(a.o) + ((grow * a.ldo + (int64_t)head * a.c.hd) << lg);
+            *reinterpret_cast<uint4*>(p + c * 16) = u;
         }
     }
     tc_fence_before();
