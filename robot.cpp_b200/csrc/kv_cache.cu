@@ -29,13 +29,24 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStre
 struct F8 {
     float v[8];
 };
-__device__ __forceinline__ F8 load8(const float* p) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+// Eight elements as they lie in memory, their values, and the largest magnitude's bits (0x7f800000 or more: an infinity or NaN).
+template <typename T>
+struct Raw8 {
+    uint4 u[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
 }
-__device__ __forceinline__ F8 load8(const __nv_bfloat16* p) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ F8 values(const Raw8<float>& r) {
+    return F8{{__uint_as_float(r.u[0].x), __uint_as_float(r.u[0].y), __uint_as_float(r.u[0].z), __uint_as_float(r.u[0].w),
+               __uint_as_float(r.u[1].x), __uint_as_float(r.u[1].y), __uint_as_float(r.u[1].z), __uint_as_float(r.u[1].w)}};
+}
+__device__ __forceinline__ F8 values(const Raw8<__nv_bfloat16>& x) {
+    const uint32_t w[4] = {x.u[0].x, x.u[0].y, x.u[0].z, x.u[0].w};
     F8 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -43,6 +54,18 @@ __device__ __forceinline__ F8 load8(const __nv_bfloat16* p) {
         r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
     return r;
+}
+__device__ __forceinline__ uint32_t magnitude(const Raw8<float>& r) {
+    uint32_t b = 0;
+    const F8 x = values(r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b = max(b, __float_as_uint(x.v[j]) & 0x7fffffffu);
+    return b;
+}
+__device__ __forceinline__ uint32_t magnitude(const Raw8<__nv_bfloat16>& r) {
+    const uint32_t m = 0x7fff7fffu;
+    const uint32_t b = __vmaxu2(__vmaxu2(r.u[0].x & m, r.u[0].y & m), __vmaxu2(r.u[0].z & m, r.u[0].w & m));
+    return max(b << 16, b & 0xffff0000u);
 }
 __device__ __forceinline__ void store8(float* p, const F8& x) {
     reinterpret_cast<float4*>(p)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
@@ -191,13 +214,14 @@ __device__ __forceinline__ uint2 codes_of(const F8& x, float s) {
         } else {
             w[i] = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[i] |= ((uint32_t)(int)fminf(fmaxf(roundf(p[j]), -127.0f), 127.0f) & 0xffu) << (8 * j);
+            for (int j = 0; j < 4; ++j)  // |p| + 1/2 rounded towards zero has the whole part of the exact sum; |p| < 127.5
+                w[i] |= ((uint32_t)(int)__fadd_rz(p[j], copysignf(0.5f, p[j])) & 0xffu) << (8 * j);
         }
     }
     return make_uint2(w[0], w[1]);
 }
 
-// LANES lanes share one (token, key or value, head), eight values each. A warp takes kFlight heads for each of its 32 / LANES
+// LANES (4, 8 or 16) lanes share one (token, key or value, head), eight values each. A warp takes kFlight heads for each of its 32 / LANES
 // groups from one token's 2 kv_heads: all loads are in flight before the first is used.
 constexpr int kFlight = 4;
 template <typename T, bool E4M3, int LANES>
@@ -214,14 +238,14 @@ kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restr
     griddep_launch();
     if (m >= M) return;
     const int64_t slot = slots[m];  // looked at when the rows are on their way
-    F8 x[kFlight];
+    const int end = heads - (f0 - g);  // the warp's steps end there
+    Raw8<T> x[kFlight];
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
         const int f = f0 + i * step;
+        x[i] = Raw8<T>{};
         if (f < heads && d < c.hd)
             x[i] = load8(f < c.kv_heads ? k + m * ldk + (int64_t)f * c.hd + d : v + m * ldv + (int64_t)(f - c.kv_heads) * c.hd + d);
-        else
-            x[i] = F8{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}};
     }
     if (slot < 0) return;
     if (slot >= c.n_pages << c.page_shift) {
@@ -229,26 +253,36 @@ kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restr
         return;
     }
     const int64_t row0 = (((slot >> c.page_shift) * c.kv_heads) << c.page_shift) + (slot & ((1 << c.page_shift) - 1));
+    auto row_of = [&](int f) { return row0 + ((int64_t)(f < c.kv_heads ? f : f - c.kv_heads) << c.page_shift); };
+    // the scales of the warp's heads: lane i of a group has step i's
+    uint32_t mine = 0;
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-        const int f = f0 + i * step;
-        uint32_t bits = 0;  // of the largest |x|; an infinity or a NaN is 0x7f800000 or more
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(x[i].v[j]) & 0x7fffffffu);
+        if (i * step >= end) break;
+        uint32_t bits = magnitude(x[i]);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-        if (f >= heads) continue;
-        constexpr float top = E4M3 ? 448.0f : 127.0f, by_top = 1.0f / top;
-        const bool bad = bits >= 0x7f800000u;
-        const float a = bad ? 1.0f : fmaxf(__uint_as_float(bits), 0x1p-100f);
-        uint2 codes = codes_of<E4M3>(x[i], __fdiv_rn(top, a));
-        if (bad) codes = make_uint2(0, 0);
+        if (lane == i) mine = bits;
+    }
+    constexpr float top = E4M3 ? 448.0f : 127.0f, by_top = 1.0f / top;
+    const bool bad = mine >= 0x7f800000u;
+    const float a = bad ? 1.0f : fmaxf(__uint_as_float(mine), 0x1p-100f);
+    const float up = bad ? 0.0f : __fdiv_rn(top, a);
+    if (lane < kFlight && f0 + lane * step < heads) {
         // a / top, correctly rounded: the quotient by the rounded reciprocal, corrected once by its exact remainder
         const float q0 = __fmul_rn(a, by_top), quotient = __fmaf_rn(__fmaf_rn(-q0, top, a), by_top, q0);
-        const bool is_v = f >= c.kv_heads;
-        const int64_t row = row0 + ((int64_t)(is_v ? f - c.kv_heads : f) << c.page_shift);
-        if (d < c.hd) *reinterpret_cast<uint2*>((is_v ? c.v : c.k) + row * c.hd + d) = codes;
-        if (lane == 0) (is_v ? c.vs : c.ks)[row] = bad ? __int_as_float(0x7fc00000) : quotient;
+        const int f = f0 + lane * step;
+        (f < c.kv_heads ? c.ks : c.vs)[row_of(f)] = bad ? __int_as_float(0x7fc00000) : quotient;
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+        if (i * step >= end) break;
+        const int f = f0 + i * step;
+        const float by = __shfl_sync(0xffffffffu, up, i, LANES);
+        if (f >= heads || d >= c.hd) continue;
+        uint2 codes = codes_of<E4M3>(values(x[i]), by);
+        if (by == 0.0f) codes = make_uint2(0, 0);  // an infinity or a NaN in the row
+        *reinterpret_cast<uint2*>((f < c.kv_heads ? c.k : c.v) + row_of(f) * c.hd + d) = codes;
     }
 }
 
