@@ -221,9 +221,14 @@ __device__ __forceinline__ uint2 codes_of(const F8& x, float s) {
     return make_uint2(w[0], w[1]);
 }
 
-// LANES (4, 8 or 16) lanes share one (token, key or value, head), eight values each. A warp takes kFlight heads for each of its 32 / LANES
-// groups from one token's 2 kv_heads: all loads are in flight before the first is used.
-constexpr int kFlight = 4;
+// LANES (4, 8 or 16) lanes share one row (a head of a key or a value), eight values each. A warp takes one head a step for each of
+// its 32 / LANES groups, from one token's 2 kv_heads: the loads of all its steps are in flight before the first is used, and the
+// lanes of a group hold one step's scale each. 18432 bf16 tokens of 5 + 5 heads of 128 to e4m3 (the bytes alone: 10.9 us): 23.9
+// us with one step, 20.9 with two, 21.1 with four (of which the fourth is empty), 16.8 with five (4.2 TB/s), 17.0 with six; of
+// 8 + 8 heads 41, 33, 29.6, 29.8 and 30 us. What is left is issue slots and latency: 56 registers hold 32 warps an SM, and
+// 40 registers, which hold 48, took 17.8 us.
+template <int LANES>
+constexpr int kWriteSteps = LANES < 5 ? LANES : 5;
 template <typename T, bool E4M3, int LANES>
 __global__ void __launch_bounds__(256)
 kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv, int M,
@@ -239,9 +244,9 @@ kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restr
     if (m >= M) return;
     const int64_t slot = slots[m];  // looked at when the rows are on their way
     const int end = heads - (f0 - g);  // the warp's steps end there
-    Raw8<T> x[kFlight];
+    Raw8<T> x[kWriteSteps<LANES>];
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < kWriteSteps<LANES>; ++i) {
         const int f = f0 + i * step;
         x[i] = Raw8<T>{};
         if (f < heads && d < c.hd)
@@ -257,7 +262,7 @@ kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restr
     // the scales of the warp's heads: lane i of a group has step i's
     uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < kWriteSteps<LANES>; ++i) {
         if (i * step >= end) break;
         uint32_t bits = magnitude(x[i]);
 #pragma unroll
@@ -268,14 +273,14 @@ kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restr
     const bool bad = mine >= 0x7f800000u;
     const float a = bad ? 1.0f : fmaxf(__uint_as_float(mine), 0x1p-100f);
     const float up = bad ? 0.0f : __fdiv_rn(top, a);
-    if (lane < kFlight && f0 + lane * step < heads) {
+    if (lane < kWriteSteps<LANES> && f0 + lane * step < heads) {
         // a / top, correctly rounded: the quotient by the rounded reciprocal, corrected once by its exact remainder
         const float q0 = __fmul_rn(a, by_top), quotient = __fmaf_rn(__fmaf_rn(-q0, top, a), by_top, q0);
         const int f = f0 + lane * step;
         (f < c.kv_heads ? c.ks : c.vs)[row_of(f)] = bad ? __int_as_float(0x7fc00000) : quotient;
     }
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < kWriteSteps<LANES>; ++i) {
         if (i * step >= end) break;
         const int f = f0 + i * step;
         const float by = __shfl_sync(0xffffffffu, up, i, LANES);
@@ -310,6 +315,7 @@ __device__ __forceinline__ F8 values_of(uint2 u, float s) {
 }
 
 // As the write: a warp takes kFlight heads a group from one token. `parts` = 2: keys and values, 1: the one whose rows are given.
+constexpr int kFlight = 4;
 template <typename T, bool E4M3, int LANES>
 __global__ void __launch_bounds__(256)
 kv_read_kernel(KvView c, const int64_t* __restrict__ slots, int M, T* __restrict__ k, int64_t ldk, T* __restrict__ v, int64_t ldv,
@@ -372,7 +378,7 @@ cudaError_t rope_typed(const void* x, int64_t ldx, int64_t M, int n_heads, int h
 template <typename T, bool E4M3, int LANES>
 cudaError_t write_typed(const KvView& c, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t M,
                         const int64_t* slots, cudaStream_t st) {
-    const int per = (int)ceil_div(2 * c.kv_heads, kFlight * (32 / LANES));
+    const int per = (int)ceil_div(2 * c.kv_heads, kWriteSteps<LANES> * (32 / LANES));
     return launch_pdl(kv_write_kernel<T, E4M3, LANES>, dim3((unsigned)ceil_div(M * per, 8)), dim3(256), st, c,
                       static_cast<const T*>(k), ldk, static_cast<const T*>(v), ldv, (int)M, slots, per);
 }
