@@ -26,6 +26,8 @@
 //
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
 // MMAs are issued, those in flight are waited for, and tensor memory is freed.
+#include <algorithm>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -44,12 +46,16 @@ constexpr int kBlock = kKeys * 128;          // bytes of 128 rows x 64 fp16 valu
 struct Rows {
     int lo, n, len, rows;  // first query row, query rows, keys, (token, head of group) rows that this pass takes
 };
+constexpr int kWide = 0x1000;
 struct Misc {
     float ks[4][kKeys];        // key scales of four tiles in flight, times the factor that takes scores to log2 units
     float vs[4][kKeys];        // value scales
     float vn[4][kKeys];        // value scales over the power of two above the largest finite one of their 32 keys
-    int vexp[4][kConvWarps];   // that one's biased exponent, 1..252
-    uint32_t there[4][kConvWarps];  // keys that exist
+    // [half] keys that exist of its two times 32, and that scale's biased exponents, 1..252, with kWide where scores may pass 2^24
+    struct alignas(16) {
+        uint32_t there[2];
+        int vexp[2];
+    } of[4][2];
     float om[2][kRows];        // [group][row] reference of the row's outputs: of the exponentials,
     int ov[2][kRows];          // and of the value scales
     float l[2][2][kRows];      // [group][half of the row's keys][row]
@@ -57,7 +63,8 @@ struct Misc {
     int64_t scan[kThreads / 32];
     int64_t found[2];
     Rows seq;                  // that sequence
-    float big[kSoftWarps];
+    float big[kSoftWarps];     // largest finite element of the warp's query rows
+    uint32_t row_big[2 * kRows];  // and of each row, as bits
     uint32_t tmem;
     int abort;
 };
@@ -351,12 +358,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
     const int all_tiles = (most + kKeys - 1) / kKeys;
     const int t0 = (unsigned)(all_tiles * split) / (unsigned)splits, nt = (unsigned)(all_tiles * (split + 1)) / (unsigned)splits - t0;
 
-    // The power of two that all query rows share: the largest finite element goes to [2^14, 2^15).
+    // The power of two that the block's query rows share: the largest finite element goes to [2^14, 2^15).
     auto common_up = [&]() {
         float big = ms->big[0];
 #pragma unroll
         for (int i = 1; i < kSoftWarps; ++i) big = fmaxf(big, ms->big[i]);
         return min(253, 268 - (__float_as_int(big) >> 23));
+    };
+
+    // A row far below it has its own, so that it keeps its bits beside a huge one (fp16 parts end at 2^-24); its scores are
+    // brought level where they are read.
+    auto up_of_row = [&](int common, int row) {
+        const uint32_t bits = ms->row_big[row];
+        const int own = min(253, 268 - (int)(bits >> 23));
+        return bits == 0 || own - common <= 12 ? common : own;
     };
 
     if (warp >= kSoftWarps) {
@@ -460,14 +475,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 wait(ms, &ms->qfull, 0);
                 rf = __fmul_rn(pow2_biased(254 - common_up()), a.scale_log2e);
             }
-            ms->ks[sc][cw * 32 + lane] = __fmul_rn(ksc, rf);
+            const float kf = __fmul_rn(ksc, rf);
+            ms->ks[sc][cw * 32 + lane] = kf;
             ms->vs[sc][cw * 32 + lane] = vsc;
             int e = __float_as_int(fabsf(vsc)) >> 23;
             e = __reduce_max_sync(0xffffffffu, e == 255 ? 1 : max(1, min(252, e)));
             ms->vn[sc][cw * 32 + lane] = __fmul_rn(vsc, pow2_biased(253 - e));
+            // elements of Q are below 2^15, codes below 2^9 and 2^7
+            const bool wide = __any_sync(0xffffffffu, !(fabsf(kf) < 0x1p9f / (HDP * (E4M3 ? 512 : 128))));
             if (lane == 0) {
-                ms->vexp[sc][cw] = e;
-                ms->there[sc][cw] = pk.bits;
+                ms->of[sc][cw >> 1].vexp[cw & 1] = wide ? e | kWide : e;
+                ms->of[sc][cw >> 1].there[cw & 1] = pk.bits;
             }
             __syncwarp();
             mbar_arrive(&ms->scfull[sc]);
@@ -491,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         }
     } else {
         // ================================================================ softmax
+        int common;
         // ---- the query rows, 16 bytes a lane: two bf16 rows or one fp32 row for each warp and load
         {
             constexpr int kPer = PARTS == 2 ? 1 : 2, kQr = kBlkRows / kSoftWarps / kPer;
@@ -513,27 +532,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                     x[i] = on ? y : 0.0f;
                 }
             };
-            float big = 0.0f;
+            uint32_t big = 0;
 #pragma unroll
             for (int k = 0; k < kQr; ++k) {
                 float x[kVals];
                 values(q[k], first + k * kSoftWarps * kPer < rows && d < a.c.hd, x);
+                uint32_t bits = 0;
 #pragma unroll
                 for (int i = 0; i < kVals; ++i) {
-                    const float y = fabsf(x[i]);
-                    big = fmaxf(big, y < INFINITY ? y : 0.0f);
+                    const uint32_t y = __float_as_uint(x[i]) & 0x7fffffffu;
+                    bits = max(bits, y < 0x7f800000u ? y : 0u);
                 }
+#pragma unroll
+                for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+                if (d == 0) ms->row_big[first + k * kSoftWarps * kPer] = bits;
+                big = max(big, bits);
             }
-            big = warp_max(big);
-            if (lane == 0) ms->big[warp] = big;
+            big = __reduce_max_sync(0xffffffffu, big);
+            if (lane == 0) ms->big[warp] = __uint_as_float(big);
             asm volatile("bar.sync 1, 512;" ::: "memory");
-            const float mul = pow2_biased(common_up());
+            common = common_up();
             if (d < HDP) {
 #pragma unroll
                 for (int k = 0; k < kQr; ++k) {
                     const int r = first + k * kSoftWarps * kPer, rr = r & (kRows - 1);
                     float x[kVals];
                     values(q[k], r < rows && d < a.c.hd, x);
+                    const float mul = pow2_biased(up_of_row(common, r));
                     uint32_t hi[kVals / 2];
                     float y[kVals];
 #pragma unroll
@@ -571,8 +596,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         const int tok = a.by_group(rb);
         // a row that is not there never masks (its results are dropped)
         const int limit = !mine ? 0x7fffffff : a.causal ? sq.len - sq.n + tok + 1 : sq.len;
-        const int wmin = __reduce_min_sync(0xffffffffu, limit);
         const int n = PAIR ? nt : (nt + 1 - wg) / 2;
+        // 0, or the power of two that takes the row's scores level
+        auto drop = [&](int up) { return up - up_of_row(up, (PAIR ? wg * kRows : 0) + r); };
+        const int wmin = __reduce_min_sync(0xffffffffu, drop(common) == 0 ? limit : -1);  // keys that all of the warp's rows see as they are
+        auto level = [&](auto& x) {
+            if (wmin >= 0) return;
+            const int by = drop(common_up());
+            const float f0 = pow2_biased(127 + max(by, -120)), f1 = pow2_biased(127 + max(min(by + 120, 0), -126));
+            for (auto& v : x) v = __float_as_uint(__fmul_rn(__fmul_rn(__uint_as_float(v), f0), f1));
+        };
         float m = -INFINITY, l = 0.0f;  // reference and sum of this thread's keys
         int vref = 8;
         // ---- this stream's MMAs, issued by one of its warps: another scheduler's for each stream
@@ -623,13 +656,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             }
             __syncwarp();
             wait(ms, &ms->scfull[sc], (uint32_t)(j >> 2) & 1u);
-            const uint2 there = *reinterpret_cast<const uint2*>(&ms->there[sc][2 * half]);
+            const int4 of = *reinterpret_cast<const int4*>(&ms->of[sc][half]);
             const int key0 = (t0 + j) * kKeys + half * kHalf;
-            const bool masked = __any_sync(0xffffffffu, (there.x & there.y) != 0xffffffffu || key0 + kHalf > wmin);
+            // not plain: keys that a row does not see, rows to be brought level, or scores for which a product that is not rounded
+            // may differ from its reference by more than a half
+            const bool plain = !__any_sync(0xffffffffu, (of.x & of.y) != -1 || key0 + kHalf > wmin || ((of.z | of.w) & kWide));
             // keys of 32 that the row sees
             auto see_of = [&](int c) {
                 const int left = limit - (key0 + 32 * c);
-                return ms->there[sc][2 * half + c] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
+                return ms->of[sc][half].there[c] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
             };
             wait(ms, &ms->sfull[st], (uint32_t)i & 1u);
             tc_fence_after();
@@ -664,8 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                     lo = pack_h2(u, v);
                 }
             };
-            if (!masked) {
-                const int e = max(ms->vexp[sc][2 * half], ms->vexp[sc][2 * half + 1]);
+            if (plain) {
+                const int e = max(of.z, of.w);
                 if (e >= vref) vref = min(e + 2, 255);
                 // P of 32 keys over their scores: p = 2^(s - m + shift) times the value scales, which are over 2^(exponent + 1)
                 // of their 32 keys (one far below the reference counts as 2^-60); their sum is taken back by 2^-shift
@@ -673,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 for (int c = 0; c < 2; ++c) {
                     const float4* ksp = reinterpret_cast<const float4*>(&ms->ks[sc][half * kHalf + 32 * c]);
                     const float4* vnp = reinterpret_cast<const float4*>(&ms->vn[sc][half * kHalf + 32 * c]);
-                    const int shift = max(-60, ms->vexp[sc][2 * half + c] + 7 - vref);
+                    const int shift = max(-60, ms->of[sc][half].vexp[c] + 7 - vref);
                     const float most = pow2_biased(127 + 8 + shift);
                     uint32_t x[32];
                     float sum;
@@ -736,6 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                     uint32_t x[16];
                     tmem_ld_x16(sbuf + 16 * c, x);
                     wait_ld(x);
+                    level(x);
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const float u = __fmul_rn(__uint_as_float(x[k]), kp[16 * c + k]);
@@ -765,6 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                         uint32_t x[16];
                         tmem_ld_x16(sbuf + 16 * c, x);
                         wait_ld(x);
+                        level(x);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             float p[2], w[2];
@@ -772,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                             for (int q = 0; q < 2; ++q) {
                                 const int key = 16 * c + 2 * k + q;
                                 const bool on = (see >> (2 * k + q)) & 1;
-                                p[q] = on ? ex2(__fmaf_rn(__uint_as_float(x[2 * k + q]), kp[key], mu)) : 0.0f;
+                                p[q] = on ? ex2(__fadd_rn(__fmul_rn(__uint_as_float(x[2 * k + q]), kp[key]), mu)) : 0.0f;
                                 w[q] = on ? __fmul_rn(p[q], __fmul_rn(vp[key], vmul)) : 0.0f;
                             }
                             sum = __fadd_rn(sum, __fadd_rn(p[0], p[1]));
@@ -1025,7 +1062,9 @@ cudaError_t launch_typed(const KvAttnArgs& a, int splits, cudaStream_t st) {
     const size_t smem = kSmem<HDP, PARTS, PAIR>;
     const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
-    const int64_t units = a.M * a.group / (PAIR ? 2 * kRows : kRows) + a.batch;  // blocks of rows at most
+    // blocks of rows at most: one more than whole ones for each sequence that has rows enough
+    const int64_t units = a.M * a.group / (PAIR ? 2 * kRows : kRows) + std::min<int64_t>(a.batch, a.M * a.group / (a.min_rows + 1));
+    if (units == 0) return cudaSuccess;
     return launch_pdl(kernel, units * a.c.kv_heads * splits, kThreads, smem, st, a, (int)units, splits);
 }
 template <int HDP, bool E4M3>

@@ -606,6 +606,127 @@ def test_attention_captured_replayed_and_on_two_streams(b2s, prefix):
     b.check(runs[1][1])
 
 
+LONG = [  # new, keys, heads, kv heads, hd: several row blocks, pairs of them (bf16), cut keys, odd tails
+    ([300], [1500], 2, 2, 64), ([520, 3, 257], [3000, 40, 700], 8, 2, 128), ([1100], [1100], 4, 1, 112), ([65], [4096], 2, 1, 32),
+    ([129], [130], 3, 3, 96), ([96, 1, 96], [2049, 2049, 127], 6, 1, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("new,keys,heads,hkv,hd", LONG)
+@pytest.mark.parametrize("dtype,code", [(F32, E4M3), (BF16, I8)])
+def test_attention_many_rows_on_long_sequences(b2s, new, keys, heads, hkv, hd, dtype, code):
+    c = Case(7 + hd + sum(keys), new, keys, heads, hkv, hd, 32, dtype, code, extra_rows=5)
+    o = c.run()
+    ok(b2s)
+    c.check(o)
+    assert torch.equal(c.run(), o)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 4, 40, 150])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("down", [False, True])
+def test_attention_scores_that_grow_or_shrink_along_the_keys(b2s, rows, dtype, down):
+    """Keys whose scales go over four decades along the sequence: the softmax reference is raised in most tiles, and with a
+    shared prefix the two parts have far references."""
+    for prefix in (0, 400):
+        c = Case(91 + rows, [rows], [700], 8, 2, 128, 16, dtype, I8, prefix=prefix, scale=0.4)
+        for pages, n in ((c.prefix_pages, prefix), (c.pages[0, :44], 700)):
+            if n:
+                ramp = torch.logspace(-3, 1, 16 * len(pages), device="cuda").view(-1, 1, 16)
+                c.cache.k_scale[pages.long()] *= ramp.flip(0, 2) if down else ramp
+                c.cache.v_scale[pages.long()] *= ramp.flip(0, 2)
+        o = c.run()
+        ok(b2s)
+        c.check(o)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [5, 160])
+def test_attention_rows_of_far_magnitudes(b2s, dtype, rows):
+    """Query rows of one block over 60 decades: each keeps its own precision. Rows far above the rest have sharp scores."""
+    for big in (1e4, 1e28):
+        c = Case(93, [rows], [300], 8, 2, 64, 16, dtype, E4M3)
+        by = torch.ones(rows, 1, device="cuda")
+        by[::7] = big
+        by[3::7] = 1 / big
+        by[4::11] = 0.0
+        c.q = (c.q.float() * by).to(dtype)
+        o = c.run()
+        ok(b2s)
+        c.check(o)
+
+
+@gpu
+def test_attention_huge_and_tiny_queries_under_a_scale(b2s):
+    for sharp, scale in ((1e30, 1e-31), (1e-30, 1e29)):
+        for code in (I8, E4M3):
+            c = Case(95, [2, 80], [200, 150], 4, 2, 128, 16, F32, code, scale=scale, sharp=sharp)
+            o = c.run()
+            ok(b2s)
+            c.check(o)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_with_another_max_q(b2s, dtype):
+    """max_q chooses kernels: too small or too large, the results stay within their bounds."""
+    for prefix in (0, 90):
+        c = Case(97, [1, 100, 0, 17], [30, 260, 5, 400], 12, 3, 128, 16, dtype, E4M3, prefix=prefix)
+        for max_q in (0, 1, 17, 100, 5000):
+            c.batch = kv.Batch(c.q_start, c.kv_len, c.pages, max_q)
+            o = c.run()
+            ok(b2s)
+            c.check(o)
+
+
+@gpu
+@pytest.mark.parametrize("prefix", [4096, 4097])
+def test_attention_prefix_on_both_sides_of_its_rule(b2s, prefix):
+    """8 sequences x 8 heads x one block of rows x 128 steps is the last prefix that is read with the own tokens."""
+    c = Case(99, [1, 2, 1, 1, 2, 1, 1, 1], [3, 40, 0, 17, 1, 9, 300, 64], 32, 8, 64, 64, F32, I8, prefix=prefix)
+    o = c.run()
+    ok(b2s)
+    c.check(o)
+    assert torch.equal(c.run(), o)
+
+
+@gpu
+def test_attention_graphs_that_share_a_workspace(b2s):
+    """Two captured calls, of few rows and of many with cut keys, on one workspace, replayed in turn on one stream."""
+    a = Case(101, [1, 1, 2], [900, 30, 64], 20, 5, 128)
+    b = Case(102, [80, 1], [700, 900], 4, 1, 128, prefix=130)
+    ws = torch.empty(max(a.workspace().numel(), b.workspace().numel()), dtype=torch.uint8, device="cuda").fill_(0xff)
+    want, s, graphs = [c.run() for c in (a, b)], torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for c in (a, b):
+        o = torch.empty_like(c.q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            c.run(o, ws)
+        graphs.append((graph, o))
+    with torch.cuda.stream(s):
+        for graph, o in graphs * 3:
+            graph.replay()
+    ok(b2s)
+    for (_, o), w in zip(graphs, want):
+        assert torch.equal(o, w)
+
+
+@gpu
+def test_attention_of_a_large_batch_with_one_prompt(b2s):
+    """The largest batch: single tokens, most without keys, and one prompt."""
+    new, keys = [1] * 16384, [0] * 16384
+    new[9000], keys[9000] = 90, 95
+    for b in range(0, 16384, 37):
+        keys[b] = 1 + b % 50
+    c = Case(103, new, keys, 8, 1, 32, 16)
+    o = c.run()
+    ok(b2s)
+    c.check(o)
+
+
 @gpu
 def test_long_cache_offsets_pass_32_bits(b2s):
     """Pages whose code rows lie past 2^32 bytes and whose scales lie past 2^31."""
