@@ -76,32 +76,39 @@ int cache_view(const b2s_kv_cache* c, b2s::KvView* v, const char* op) {
 
 // Which kernels take the rows of a call, decided from sizes that the host has. Sequences with at most kFewRows rows a
 // key/value head go to the warp-level kernel, which reads their keys once per eight rows; the others to the tensor-core
-// kernel, which reads them once per 128.
-constexpr int kFewRows = 64;
+// kernel, which reads them once per 128. Five heads of 128, int8, us with the first and with the second kernel: 16 sequences
+// of 2000 keys, 20 rows 41 and 55 (bf16 40 and 44), 32 rows 49 and 56 (47 and 45), 48 rows 66 and 57 (64 and 45), 64 rows 82 and
+// 57 (80 and 45); one sequence, 32 rows 18.2 and 18.5 (17.2 and 15.5), 64 rows 22.6 and 19.4 (21.0 and 15.9).
+constexpr int kFewRows = 32;
 struct Plan {
     bool few, many, pair;  // pair: blocks of 256 rows
     int min_rows, splits;
 };
-// The tensor-core kernel's part of a plan for M tokens of up to max_q a sequence over `keys` keys.
+// The tensor-core kernel's part of a plan for M tokens of up to max_q a sequence over `keys` keys: blocks of 128 or (bf16) 256
+// rows, and into how many shares the keys are cut where that gives less than a wave of blocks. The least estimate is taken, in
+// half tiles' time: waves x (a block's tiles of 128 keys, 2 each or 3 for 256 rows, + 8 or 12 to start and end it), + 6 for the
+// join. bf16, five heads, us with blocks of 128 and of 256 rows: one sequence of 256 rows on 2000 keys 19 and 27, 8 of 260 on
+// 2000 keys 45 and 76, 2 of 2048 on 4096 keys 144 and 119, 8 of 512 on 128 keys 23 and 18. fp32, whole keys and cut ones: 260
+// rows on 8192 keys 175 and 40, 512 on 2000 keys 54 and 27, 4096 rows of one head on 4096 keys 94 and 41.
 void plan_blocks(Plan* p, int64_t M, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
     p->many = true;
-    p->pair = bf16 && max_q * group > 128;
-    // Less than a wave of blocks: cut the keys, so that waves x (tiles of 128 keys + about four tiles' worth of starting and
-    // ending a block) is least.
-    const int block = p->pair ? 256 : 128;
-    const int64_t units = std::max<int64_t>(1, M * group / block) * kv_heads, tiles = (keys + 127) / 128;
-    int64_t best = 0;
-    p->splits = 1;
-    for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles) && units < 148; ++s) {
-        const int64_t cost = (units * s + 147) / 148 * ((tiles + s - 1) / s + 4) + (s > 1 ? 3 : 0);
-        if (s == 1 || cost < best) {
-            best = cost;
-            p->splits = s;
+    const int64_t seqs = (M + max_q - 1) / max_q, tiles = std::max<int64_t>(1, (keys + 127) / 128);
+    int64_t best = -1;
+    for (int pair = 0; pair <= (bf16 ? 1 : 0); ++pair) {
+        const int64_t units = std::max<int64_t>(1, seqs) * ((max_q * group + 128 * (1 + pair) - 1) / (128 * (1 + pair))) * kv_heads;
+        for (int s = 1; s <= 16 && s <= tiles && (s == 1 || units < 148); ++s) {
+            const int64_t cost = (units * s + 147) / 148 * ((tiles + s - 1) / s * (2 + pair) + 8 + 4 * pair) + (s > 1 ? 6 : 0);
+            if (best < 0 || cost < best) {
+                best = cost;
+                p->pair = pair != 0;
+                p->splits = s;
+            }
         }
     }
 }
 Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
     Plan p{true, false, false, 0, 1};
+    max_q = std::min(max_q, M);  // it may be any bound
     if (max_q * group <= kFewRows) return p;
     plan_blocks(&p, M, max_q, group, kv_heads, keys, bf16);
     p.few = M != batch * max_q;  // equal: every sequence has max_q rows
@@ -111,12 +118,13 @@ Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads,
 
 // A shared prefix goes through the tensor-core kernel, once for all rows, unless few rows make it cheaper to let every
 // sequence read it with its own tokens (from L2): up to kPrefixSteps steps of 32 keys and eight rows. One pass then takes the
-// place of three: 16 rows on 545 shared tokens (1440 steps) took 26 us in passes of their own.
+// place of three. 20 heads on 5, int8, us with one pass and with three: 16 rows on 545 shared tokens (1440 steps) 21.5 and 25.1,
+// 32 on 1600 (8000) 30.2 and 31.0, 64 on 800 (8000) 32.4 and 30.2, 64 on 1600 (16000) 43.9 and 32.4.
 constexpr int64_t kPrefixSteps = 8192;
 Plan plan_prefix(const Plan& own, int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t prefix_len, bool bf16) {
     Plan p{false, false, false, 0, 1};
     if (prefix_len == 0) return p;
-    if (!own.many && batch * kv_heads * ((max_q * group + 7) / 8) * ((prefix_len + 31) / 32) <= kPrefixSteps)
+    if (M == 0 || (!own.many && batch * kv_heads * ((std::min(max_q, M) * group + 7) / 8) * ((prefix_len + 31) / 32) <= kPrefixSteps))
         p.few = true;
     else
         plan_blocks(&p, M, M, group, kv_heads, prefix_len, bf16);

@@ -144,6 +144,16 @@ def test_workspace_grows_with_the_prefix(b2s):
     assert plain > 0 and shared >= plain + 64 * 20 * 130 * 4 and shared % 256 == 0
 
 
+@pytest.mark.parametrize("M,batch,max_q,heads,prefix", [
+    (0, 3, 1000, 20, 5000), (0, 0, 0, 20, 0), (0, 16384, 2 ** 31 - 1, 2 ** 31 - 8, 2 ** 20), (7, 1, 2 ** 31 - 1, 20, 2 ** 20),
+    (7, 16384, 0, 20, 2 ** 20), (2 ** 24, 1, 2 ** 24, 20, 2 ** 20)])
+def test_workspace_of_unusual_batches(b2s, M, batch, max_q, heads, prefix):
+    c, b = cache_struct(), batch_struct(batch=batch, max_q=max_q)
+    heads -= heads % 5
+    size = kv._bind().b2s_attention_kv_workspace_size(C.byref(c), C.byref(b), M, heads, prefix)
+    assert size > 0 and size <= 2 ** 24 + 33 * (M + 1) * heads * 130 * 4
+
+
 def test_binding_refuses_host_tensors_and_shapes(b2s):
     x = torch.zeros(4, 640)
     with pytest.raises(ValueError, match="CUDA"):
