@@ -88,9 +88,11 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache *cache, const b2s_kv_b
 /* o = softmax(scale * q K^T) V of every sequence's query rows over its cached tokens; q and o [M][n_heads * head_dim]
  * of `type`, query head h reads key/value head h / (n_heads / n_kv_heads). With causal != 0 query row i of n sees the
  * tokens j <= kv_len - n + i, else all. A row that sees nothing is written as zeros; rows of o outside
- * [q_start[0], q_start[batch]) are left as they were. o may be q. Scores, softmax and sums are fp32, products run on
- * the tensor cores: the 8-bit codes are exact in fp16, fp32 queries and probabilities are taken as two fp16 parts
- * (relative error 2^-22), bf16 queries exactly and their probabilities as one or two. */
+ * [q_start[0], q_start[batch]) are left as they were. o may be q. scale is finite and below 2^127.
+ * Scores, softmax and sums are fp32, products run on the tensor cores, where the 8-bit codes are exact. fp32 queries
+ * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or 2^-40 of its row's largest one), or,
+ * queries on int8 codes, as integers of 24 bits under the row's largest element; bf16 queries likewise or exactly, their
+ * probabilities as one (error 2^-11) or two parts. A query head with an infinity or a NaN is NaN; no other one is. */
 int b2s_attention_kv(const b2s_kv_cache *cache, const b2s_kv_batch *batch, int32_t type, const void *q, int64_t ldq,
                      int64_t M, int n_heads, float scale, int causal, void *o, int64_t ldo, void *workspace,
                      size_t workspace_bytes, void *stream);

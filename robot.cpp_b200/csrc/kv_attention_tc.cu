@@ -64,7 +64,7 @@ struct Misc {
     int64_t found[2];
     Rows seq;                  // that sequence
     float big[kSoftWarps];     // largest finite element of the warp's query rows
-    uint32_t row_big[2 * kRows];  // and of each row, as bits
+    uint32_t row_big[2 * kRows];  // the largest magnitude of each row, as bits
     uint32_t tmem;
     int abort;
 };
@@ -539,14 +539,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 values(q[k], first + k * kSoftWarps * kPer < rows && d < a.c.hd, x);
                 uint32_t bits = 0;
 #pragma unroll
-                for (int i = 0; i < kVals; ++i) {
-                    const uint32_t y = __float_as_uint(x[i]) & 0x7fffffffu;
-                    bits = max(bits, y < 0x7f800000u ? y : 0u);
-                }
+                for (int i = 0; i < kVals; ++i) bits = max(bits, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
                 for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
                 if (d == 0) ms->row_big[first + k * kSoftWarps * kPer] = bits;
-                big = max(big, bits);
+                big = max(big, bits < 0x7f800000u ? bits : 0u);
             }
             big = __reduce_max_sync(0xffffffffu, big);
             if (lane == 0) ms->big[warp] = __uint_as_float(big);
@@ -597,13 +594,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         // a row that is not there never masks (its results are dropped)
         const int limit = !mine ? 0x7fffffff : a.causal ? sq.len - sq.n + tok + 1 : sq.len;
         const int n = PAIR ? nt : (nt + 1 - wg) / 2;
-        // 0, or the power of two that takes the row's scores level
-        auto drop = [&](int up) { return up - up_of_row(up, (PAIR ? wg * kRows : 0) + r); };
+        // 0, or the power of two that takes the row's scores level; 1: an infinity or a NaN makes them NaN
+        auto drop = [&](int up) {
+            const int row = (PAIR ? wg * kRows : 0) + r;
+            return ms->row_big[row] >= 0x7f800000u ? 1 : up - up_of_row(up, row);
+        };
         const int wmin = __reduce_min_sync(0xffffffffu, drop(common) == 0 ? limit : -1);  // keys that all of the warp's rows see as they are
         auto level = [&](auto& x) {
             if (wmin >= 0) return;
             const int by = drop(common_up());
-            const float f0 = pow2_biased(127 + max(by, -120)), f1 = pow2_biased(127 + max(min(by + 120, 0), -126));
+            const float f0 = by > 0 ? __int_as_float(0x7fc00000) : pow2_biased(127 + max(by, -120)), f1 = pow2_biased(127 + max(min(by + 120, 0), -126));
             for (auto& v : x) v = __float_as_uint(__fmul_rn(__fmul_rn(__uint_as_float(v), f0), f1));
         };
         float m = -INFINITY, l = 0.0f;  // reference and sum of this thread's keys

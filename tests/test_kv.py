@@ -669,6 +669,31 @@ def test_attention_rows_of_far_magnitudes(b2s, dtype, rows):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("rows", [6, 160])
+def test_attention_query_heads_that_are_not_finite(b2s, dtype, code, rows):
+    """An infinity or a NaN makes its (row, head) NaN, whatever the signs of the keys, and no other one."""
+    for prefix in (0, 70):
+        c = Case(94, [rows], [rows + 20], 8, 2, 64, 16, dtype, code, prefix=prefix)
+        c.cache.k.view(torch.uint8 if code == E4M3 else I8).bitwise_and_(0x7f)  # no negative keys: one infinity gives equal signs
+        bad = [(0, 0, -math.inf), (2, 5, math.inf), (3, 7, math.nan), (rows - 1, 1, -math.inf)]
+        clean = c.q.clone()
+        for row, head, x in bad:
+            c.q[row, head * 64 + 9] = x
+        o = c.run()
+        ok(b2s)
+        o = o.view(rows, 8, 64)
+        c.q = clean
+        ref, tol = (x.view(rows, 8, 64) for x in c.reference())
+        good = torch.ones(rows, 8, dtype=torch.bool, device="cuda")
+        for row, head, _ in bad:
+            good[row, head] = False
+        assert bool(torch.isnan(o[~good]).all())
+        assert bool(((o.double() - ref).abs() <= tol)[good].all())
+
+
+@gpu
 def test_attention_huge_and_tiny_queries_under_a_scale(b2s):
     for sharp, scale in ((1e30, 1e-31), (1e-30, 1e29)):
         for code in (I8, E4M3):
