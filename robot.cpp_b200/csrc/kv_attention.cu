@@ -22,7 +22,7 @@
 // four warps take the tiles of its range in turn, each through its own ring of asynchronous copies (no block-wide
 // wait between tiles, the ring runs on across units); at a unit's end they are joined through shared memory. A unit cut
 // by a range's border leaves partial results that kv_attention_join_kernel puts together: the order is fixed by the
-// lengths alone, so results do not change from run to run.
+// lengths alone, so results do not change from run to run. Short units are not cut, and many short ones go to a warp each.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -40,8 +40,15 @@ constexpr int kTile = 32;   // keys per warp step
 constexpr int kRows = 8;    // query rows of a unit
 constexpr int kStages = 2;
 constexpr int kPerSm = 3, kMaxCtas = kPerSm * 160;
-constexpr int kMinTiles = 8;     // a block gets at least this many tiles (two steps of each warp)
-constexpr int kWholeTiles = 24;  // units that cannot have more tiles are not cut
+constexpr int kMinTiles = 8;  // a block gets at least this many tiles (two steps of each warp); 2 or 32 cost 4 x 2000 keys 20%, 60%
+// Units that cannot have more tiles are not cut: nothing is left to join. 64 x 5 units of 500 tokens 17 us against 30 cut ones, of
+// 700 20 against 29; one sequence of 700 14.6 against 14.0, of 1500 24 (not cut) against 15.
+constexpr int kWholeTiles = 24;
+// Nor are units of at most this many tiles shared by a block's warps, if they are many: 8 units > (8 + tiles) blocks. Five heads, us
+// with a unit a block and a unit a warp: 128 sequences of 30 tokens 15.3 and 10.4, 512 42 and 21; 128 of 100 17.1 and 18.2, 256
+// 26 and 20, 512 51 and 38; 128 of 300 27 and 34, 256 40.4 and 38.7, 512 77 and 69; 512 of 600 111 and 114. A warp alone takes
+// 1.4 us a tile, so few units or long ones are better shared.
+constexpr int kSoloTiles = 12;
 template <int HD>
 constexpr int kStageBytes = 2 * kTile * HD + 2 * kTile * 4 + 128;  // K, V codes, scales, which keys are there
 template <int HD>
@@ -202,8 +209,10 @@ struct Ranges {
     }
 };
 
-// All threads: the total of tiles, how many blocks share them, and the place of block c's first tile (c < ctas).
-__device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, Place& place, int64_t* sh, Place* sh_place) {
+// All threads: the total of tiles, how many workers (blocks, or N = kWarps warps each) share them, and the places of the first
+// tiles of the block's workers c, c + 1, ... below ctas.
+template <int N>
+__device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, int64_t* sh, Place (&sh_place)[N]) {
     int64_t total = 0, w = 0, incl = 0, sum;
     for (int base = 0; base < a.batch; base += kThreads) {
         const int b = base + threadIdx.x;
@@ -214,25 +223,30 @@ __device__ __forceinline__ Ranges find_range(const KvAttnArgs& a, int c, Place& 
     Ranges r;
     r.total = total;
     const int64_t want = a.whole_units ? total : (total + kMinTiles - 1) / kMinTiles;
-    r.ctas = (int)(want < gridDim.x ? want : gridDim.x);
+    r.ctas = (int)(want < N * gridDim.x ? want : N * gridDim.x);
     if (c >= r.ctas) return r;
     r.share = quotient(total, r.ctas);
     r.more = (int)(total - r.share * r.ctas);
-    const int64_t target = r.start(c);
+    auto look = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t target = r.start(c + i);
+            if (c + i < r.ctas && target >= incl - w && target < incl) sh_place[i] = Place{b, target - (incl - w)};
+        }
+    };
     if (a.batch <= kThreads) {
-        if (target >= incl - w && target < incl) *sh_place = Place{(int)threadIdx.x, target - (incl - w)};
+        look(threadIdx.x);
     } else {
         int64_t before = 0;
         for (int base = 0; base < a.batch; base += kThreads) {
             const int b = base + threadIdx.x;
             w = b < a.batch ? work_of(seq_of(a, b), a) : 0;
             incl = block_scan(w, sh, sum) + before;
-            if (target >= incl - w && target < incl) *sh_place = Place{b, target - (incl - w)};
+            look(b);
             before += sum;
         }
     }
     __syncthreads();
-    place = *sh_place;
     return r;
 }
 
@@ -312,7 +326,8 @@ __device__ __forceinline__ void finish(const KvAttnArgs& a, int64_t row, int hea
 }
 
 // ---------------------------------------------------------------- the pass over the keys
-template <int HD, bool E4M3, bool PREFIX>
+// SOLO: a unit's tiles belong to one warp, and nothing is joined.
+template <int HD, bool E4M3, bool PREFIX, bool SOLO>
 __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const KvAttnArgs a) {
     constexpr int kChunks = HD / 16;          // 16-byte chunks of a code row
     constexpr int kStage = kStageBytes<HD>;
@@ -322,22 +337,29 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
     constexpr int kOstride = HD / 4 + 4, kOrow = 4 * kOstride;  // padded output rows in shared memory (floats)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t sh_scan[kWarps];
-    __shared__ Place sh_place;
+    constexpr int kTeam = SOLO ? 1 : kWarps, kTeams = kWarps / kTeam;  // warps that share a unit's tiles
+    __shared__ Place sh_place[kTeams];
     __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
-    __shared__ Walk sh_load[kWarps], sh_walk[2];
+    __shared__ Walk sh_load[kWarps], sh_walk[kTeams][2];
     __shared__ int sh_free[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     griddep_wait();
     griddep_launch();
 
-    Place place;
-    const Ranges rg = find_range(a, blockIdx.x, place, sh_scan, &sh_place);
+    const int team = SOLO ? warp : 0, member = SOLO ? 0 : warp, worker = blockIdx.x * kTeams + team;
+    auto sync = [&]() {
+        if (SOLO)
+            __syncwarp();
+        else
+            __syncthreads();
+    };
+    const Ranges rg = find_range(a, blockIdx.x * kTeams, sh_scan, sh_place);
     Border* border = reinterpret_cast<Border*>(a.part + (int64_t)2 * kMaxCtas * kPart<128>) + blockIdx.x;
-    if ((int)blockIdx.x >= rg.ctas) {
-        if (threadIdx.x == 0) border->pieces = 0;
+    if (worker >= rg.ctas) {
+        if (!SOLO && threadIdx.x == 0) border->pieces = 0;
         return;
     }
-    const int64_t first = rg.start(blockIdx.x), last = rg.start(blockIdx.x + 1);
+    const int64_t first = rg.start(worker), last = rg.start(worker + 1);
     uint8_t* ring = smem + warp * (kStages * kStage);
     const uint32_t ring_u = smem_u32(ring);
 
@@ -345,17 +367,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
     // for the block. Registers hold what a tile needs.
     if (lane == 0) {
         Walk w;
-        w.begin(a, place, first, last);
+        w.begin(a, sh_place[team], first, last);
         sh_load[warp] = w;
-        if (warp == 0) sh_walk[0] = w;
+        if (member == 0) sh_walk[team][0] = w;
     }
-    __syncthreads();
+    sync();
 
     // ---- loader: the warp's tiles in order, one ahead with the page numbers
     int lt, lt_end, l_len, l_head, l_seq;
     auto take_load = [&]() {
         const Walk& w = sh_load[warp];
-        lt = w.t0 + warp;
+        lt = w.t0 + member;
         lt_end = w.t1;
         l_len = w.s.len;
         l_head = w.u / w.s.row_tiles;
@@ -426,13 +448,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
             cp_async4(st + 2 * kTile * HD + lane * 4, a.c.ks + row, on);
             cp_async4(st + 2 * kTile * HD + kTile * 4 + lane * 4, a.c.vs + row, on);
             if (lane == 0) *reinterpret_cast<uint32_t*>(ring + stage * kStage + 2 * kTile * HD + 2 * kTile * 4) = bits;
-            lt += kWarps;
+            lt += kTeam;
             fetch();
         }
         cp_commit();
     };
-    if (threadIdx.x == 0) {
-        const Walk& cw = sh_walk[0];
+    if (!SOLO && threadIdx.x == 0) {
+        const Walk& cw = sh_walk[0][0];
         Border bd{0, 0, 0, 0, 0, 0};
         if (cw.t0 > 0) {  // this block's start cuts a unit
             const int64_t unit = first - cw.t0, before = rg.start(blockIdx.x - 1);
@@ -451,9 +473,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
     fetch();
     int it = 0;  // tiles this warp has taken
 
-    for (int seg = 0; !sh_walk[seg & 1].done(); ++seg) {
+    for (int seg = 0; !sh_walk[team][seg & 1].done(); ++seg) {
         const bool head_seg = seg == 0;
-        const Walk& cw = sh_walk[seg & 1];
+        const Walk& cw = sh_walk[team][seg & 1];
         const int h = cw.u / cw.s.row_tiles, row0 = (cw.u - h * cw.s.row_tiles) * kRows;
         const int rows = min(kRows, cw.s.n * a.group - row0), seg_end = cw.t1;
         // ---- the query row of this thread's group: its share [t * HD / 4, (t + 1) * HD / 4), as fp32 words
@@ -533,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
         float m = -INFINITY, l = 0.0f;
         int vref = 15;  // biased exponent above every value scale so far
 
-        for (int tile = cw.t0 + warp; tile < seg_end; tile += kWarps, ++it) {
+        for (int tile = cw.t0 + member; tile < seg_end; tile += kTeam, ++it) {
             cp_wait<kStages - 2>();
             __syncwarp();
             issue((it + kStages - 1) % kStages);
@@ -655,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
             }
         }
 
-        // ---- join the four warps: every warp's free ring stage holds its outputs (the stage that its next copy fills)
+        // ---- join the unit's warps: every warp's free ring stage holds its outputs (the stage that its next copy fills)
         l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 1));
         l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 2));
         if (t == 0) {
@@ -680,22 +702,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
                 }
         }
         if (lane == 0) sh_free[warp] = free_stage;
-        if (threadIdx.x == 0) {  // the next segment; everybody reads it behind the last barrier of this one
+        if (member == 0 && lane == 0) {  // the next segment; everybody reads it behind the last barrier of this one
             Walk w = cw;
             w.advance(a);
-            sh_walk[(seg + 1) & 1] = w;
+            sh_walk[team][(seg + 1) & 1] = w;
         }
-        __syncthreads();
-        {
+        sync();
+#pragma unroll 1
+        for (int row = SOLO ? lane / 16 : threadIdx.x / 16; row < kRows; row += 2 * kTeam) {
             constexpr int N = HD / 16;
-            const int row = threadIdx.x / 16, d = (threadIdx.x % 16) * N;
+            const int d = (threadIdx.x % 16) * N;
             float mm = -INFINITY, ll = 0.0f, o[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) o[j] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_m[w][row]);
+            for (int w = team; w < team + kTeam; ++w) mm = fmaxf(mm, sh_m[w][row]);
 #pragma unroll 1
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = team; w < team + kTeam; ++w) {
                 const float mw = sh_m[w][row], f = mw == -INFINITY ? 0.0f : ex2(__fsub_rn(mw, mm));
                 const float* ob = reinterpret_cast<const float*>(smem + (w * kStages + sh_free[w]) * kStage) + row * kOrow +
                                   (d / (HD / 4)) * kOstride + d % (HD / 4);
@@ -703,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
 #pragma unroll
                 for (int j = 0; j < N; ++j) o[j] = __fmaf_rn(ob[j], f, o[j]);
             }
-            if (cw.t0 == 0 && cw.t1 == cw.s.tiles) {
+            if (SOLO || (cw.t0 == 0 && cw.t1 == cw.s.tiles)) {
                 if (row < rows && d < a.c.hd) {
                     const int r = row0 + row, i = a.by_group(r);
                     finish<N>(a, cw.s.lo + (int64_t)i, h * a.group + (r - i * a.group), d, mm, ll, o);
@@ -719,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) kv_attention_kernel(const Kv
                 }
             }
         }
-        __syncthreads();
+        sync();
     }
     cp_wait<0>();
 }
@@ -812,14 +835,18 @@ cudaError_t launch_args(K kernel, int grid, int block, size_t smem, const KvAttn
 template <int HD, bool E4M3, bool PREFIX>
 cudaError_t launch_typed(const KvAttnArgs& a, cudaStream_t st) {
     const size_t smem = (size_t)kWarps * kStages * kStageBytes<HD>;
-    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kv_attention_kernel<HD, E4M3, PREFIX>), smem);
-    if (e != cudaSuccess) return e;
     const int grid = resident_blocks();
     KvAttnArgs b = a;
     b.prefix_pad = (int)round_up(a.prefix_len, kTile);
     b.whole_units = b.prefix_pad + (a.max_pages << a.c.page_shift) <= kWholeTiles * kTile;
-    if ((e = launch_args(kv_attention_kernel<HD, E4M3, PREFIX>, grid, kThreads, smem, b, st)) != cudaSuccess || b.whole_units)
-        return e;
+    // units, as far as the host knows: the longer sequences of a mixed batch are not among them
+    const int64_t mean = ceil_div(a.M * a.group, a.batch), each = mean > a.max_rows ? 1 : ceil_div(mean, kRows);
+    const int64_t tiles = (b.prefix_pad + (a.max_pages << a.c.page_shift)) / kTile;
+    const bool solo = b.whole_units && tiles <= kSoloTiles && 8 * each * a.batch * a.c.kv_heads > (8 + tiles) * grid;
+    const auto kernel = solo ? kv_attention_kernel<HD, E4M3, PREFIX, true> : kv_attention_kernel<HD, E4M3, PREFIX, false>;
+    cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    if ((e = launch_args(kernel, grid, kThreads, smem, b, st)) != cudaSuccess || b.whole_units) return e;
     return launch_args(kv_attention_join_kernel<HD>, grid - 1, kJoinThreads, 0, b, st);
 }
 template <int HD, bool E4M3>

@@ -728,6 +728,21 @@ def test_attention_prefix_on_both_sides_of_its_rule(b2s, prefix):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,code,hd", [(F32, I8, 128), (BF16, E4M3, 128), (F32, E4M3, 80), (BF16, I8, 48)])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_attention_many_short_sequences(b2s, dtype, code, hd, prefix):
+    """Units of few tiles that a warp takes alone: more of them than resident warps, several a warp, ragged, some empty."""
+    g = np.random.default_rng(17)
+    new = [int(x) for x in g.integers(0, 4, 900)]
+    keys = [int(x) for x in g.integers(0, 66, 900)]
+    c = Case(107, new, keys, 9, 3, hd, 16, dtype, code, prefix=prefix, extra_rows=3)
+    o = c.run()
+    ok(b2s)
+    c.check(o)
+    assert torch.equal(c.run(), o)
+
+
+@gpu
 def test_attention_graphs_that_share_a_workspace(b2s):
     """Two captured calls, of few rows and of many with cut keys, on one workspace, replayed in turn on one stream."""
     a = Case(101, [1, 1, 2], [900, 30, 64], 20, 5, 128)
