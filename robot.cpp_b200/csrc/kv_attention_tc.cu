@@ -24,6 +24,12 @@
 // outputs have one reference; its two streams commit their products to it in turn, and whoever finds the other's reference
 // changed brings its own probabilities, or the outputs, under the larger one.
 //
+// Measured: 2 x up to 2048 bf16 tokens on 8192 e4m3 ones, causal, 32 heads on 8 of 128: 567 us, 626 TFLOP/s of the 1640 that a
+// library product reaches; 1024 tokens on 4096 with 20 heads on 5: 119 us (fp32, two products for one, 183 us). Tensor cores
+// and exponentials are each a third busy and issue slots a half: a stream's chain of 6200 clocks for 64 keys bounds it, and
+// tensor memory has no columns for more streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the
+// first codes) and end (6,000): 8 prompts of 288 fp32 tokens take 58 us.
+//
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
 // MMAs are issued, those in flight are waited for, and tensor memory is freed.
 #include <algorithm>

@@ -1,7 +1,9 @@
 // kv_cache.cu -- what happens to new tokens before and after attention: rotary positions with several axes, the
 // quantised write into the paged cache, and the read back.
 //
-// All three move bytes: their floor is HBM traffic (rope 2 x rows, write rows + codes, read codes + rows).
+// All three move bytes: their floor is HBM traffic (rope 2 x rows, write rows + codes, read codes + rows). Measured (the copy
+// rate is 6.5 TB/s): rope, 16384 bf16 rows of 25 heads of 128, 37.8 us, 5.6 TB/s; write, 18432 bf16 tokens of 5 + 5 heads to
+// e4m3, 16.8 us, 4.2 TB/s; read, 65537 tokens of 8 + 8 e4m3 heads to bf16, 76 us, 5.3 TB/s; a few rows 2-3 us, one launch.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -119,7 +121,8 @@ __device__ __forceinline__ float2 cos_sin(int pos, double turn) {
 
 // A warp turns one row's heads [h0, h0 + heads): per_head lanes of W pairs (16 bytes and the 16 half a head on) hold their
 // cosines and sines in registers for all of them, 32 / per_head heads side by side, kRopeFlight of those steps in flight; the
-// angles are formed while the first ones arrive.
+// angles are formed while the first ones arrive. One thread a pair of values had taken 50.8 us for the
+// 16384 rows.
 constexpr int kRopeFlight = 4;
 template <typename T, int W>
 __global__ void __launch_bounds__(256)
@@ -314,7 +317,7 @@ __device__ __forceinline__ F8 values_of(uint2 u, float s) {
     return r;
 }
 
-// As the write: a warp takes kFlight heads a group from one token. `parts` = 2: keys and values, 1: the one whose rows are given.
+// As the write: a warp takes kFlight heads a group from one token; a thread's one load at a time had taken 238 us for the 65537. `parts` = 2: keys and values, 1: the one whose rows are given.
 constexpr int kFlight = 4;
 template <typename T, bool E4M3, int LANES>
 __global__ void __launch_bounds__(256)
