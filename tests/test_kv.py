@@ -144,6 +144,13 @@ def test_workspace_grows_with_the_prefix(b2s):
     assert plain > 0 and shared >= plain + 64 * 20 * 130 * 4 and shared % 256 == 0
 
 
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, 2.0 ** 127, -3e38])
+def test_scales_without_room_are_refused(b2s, scale):
+    c, b = cache_struct(), batch_struct()
+    assert kv._bind().b2s_attention_kv(C.byref(c), C.byref(b), 0, P, 2560, 4, 20, scale, 1, P, 2560, P, 1 << 40, None) == INVALID
+    assert "scale" in b2s.last_error()
+
+
 @pytest.mark.parametrize("M,batch,max_q,heads,prefix", [
     (0, 3, 1000, 20, 5000), (0, 0, 0, 20, 0), (0, 16384, 2 ** 31 - 1, 2 ** 31 - 8, 2 ** 20), (7, 1, 2 ** 31 - 1, 20, 2 ** 20),
     (7, 16384, 0, 20, 2 ** 20), (2 ** 24, 1, 2 ** 24, 20, 2 ** 20)])
