@@ -92,7 +92,7 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache *cache, const b2s_kv_b
  * Scores, softmax and sums are fp32, products run on the tensor cores, where the 8-bit codes are exact. fp32 queries
  * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or 2^-40 of its row's largest one), or,
  * queries on int8 codes, as integers of 24 bits under the row's largest element; bf16 queries likewise or exactly, their
- * probabilities as one (error 2^-11) or two parts. A query head with an infinity or a NaN is NaN; no other one is. */
+ * probabilities as fp32 ones. A query head with an infinity or a NaN is NaN; no other one is. */
 int b2s_attention_kv(const b2s_kv_cache *cache, const b2s_kv_batch *batch, int32_t type, const void *q, int64_t ldq,
                      int64_t M, int n_heads, float scale, int causal, void *o, int64_t ldo, void *workspace,
                      size_t workspace_bytes, void *stream);

@@ -2,9 +2,12 @@
 // tensor cores: prompts, chunks of long prompts, and a batch's rows on a shared prefix.
 //
 // Mathematics as in kv_attention.cu: the 8-bit codes are exact in fp16; query rows scaled by a power of two are one
-// (bf16) or two (fp32) fp16 parts, and so are the probabilities times the value scale. One MMA a part:
+// (bf16) or two (fp32) fp16 parts, and the probabilities times the value scale are two. One MMA a part:
 //   S = sum over parts Q_part K^T,  O += sum over parts P_part V   (fp32 accumulation in tensor memory).
-// Floor: 4 * pairs * hd operations a head times the parts, at the fp16 rate; next to it the exponentials, 16 a clock and SM.
+// One part of P would round each weight to 2^-11: 2 to 5% of bf16 outputs then came out a step off (a chunk of 2048 tokens on
+// 8192 took 572 us with it and takes 722 with two).
+// Floor: 2 * pairs * hd operations a head for each part of Q and P, at the fp16 rate; next to it the exponentials, 16 a clock
+// and SM.
 //
 // A block takes rows (tokens x the heads of a group) of one sequence and key/value head and walks its keys in tiles of 128.
 // Four warps bring codes from the pages, unpack them and store fp16 tiles in the 128-byte swizzled layout that serves K as a
@@ -24,10 +27,9 @@
 // outputs have one reference; its two streams commit their products to it in turn, and whoever finds the other's reference
 // changed brings its own probabilities, or the outputs, under the larger one.
 //
-// Measured: 2 x up to 2048 bf16 tokens on 8192 e4m3 ones, causal, 32 heads on 8 of 128: 567 us, 626 TFLOP/s of the 1640 that a
-// library product reaches; 1024 tokens on 4096 with 20 heads on 5: 119 us (fp32, two products for one, 183 us). Tensor cores
-// and exponentials are each a third busy and issue slots a half: a stream's chain of 6200 clocks for 64 keys bounds it, and
-// tensor memory has no columns for more streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the
+// Measured: 2 x up to 2048 bf16 tokens on 8192 e4m3 ones, causal, 32 heads on 8 of 128: 722 us, 492 TFLOP/s of the 1640 that a
+// library product reaches (738 with P's second part counted); 1024 tokens on 4096 with 20 heads on 5: 149 us (fp32, whose Q has
+// two parts too, 183 us). A stream's chain for 64 keys bounds it, no unit does, and tensor memory has no columns for more streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the
 // first codes) and end (6,000): 8 prompts of 288 fp32 tokens take 58 us.
 //
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
@@ -644,8 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             const uint32_t vt = smem_u32(sV) + (j & 1) * kTileBytes + half * (kHalf * 128);
             const uint64_t vd = desc_mn_sw128(vt);
 #pragma unroll
-            for (int k = 0; k < PARTS * (kHalf / 16); ++k) {  // P of 32 keys: 16 columns of the large parts, 16 of the small ones
-                const int part = PARTS - 1 - k / (kHalf / 16), s = k % (kHalf / 16);
+            for (int k = 0; k < 2 * (kHalf / 16); ++k) {  // P of 32 keys: 16 columns of the large parts, 16 of the small ones
+                const int part = 1 - k / (kHalf / 16), s = k % (kHalf / 16);
                 mma_ts(o0, s0 + (s >> 1) * 32 + part * 16 + (s & 1) * 8, vd + (s * 2048 >> 4), idesc_f16(HDP, true),
                        k > 0 ? 1u : i + half > 0 ? 1u : 0u);
             }
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 tc_wait_st();
                 const __half2 f2h = __float2half2_rn(f);
 #pragma unroll 1
-                for (int c = 0; c < 32 * chunks; c += PARTS == 1 ? 32 : 16) {
+                for (int c = 0; c < 32 * chunks; c += 16) {
                     uint32_t x[16];
                     tmem_ld_x16(sbuf + c, x);
                     wait_ld(x);
@@ -699,11 +701,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 float u, v;
                 unf2(w, u, v);
                 hi = pack_h2(u, v);
-                if (PARTS == 2) {
-                    const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                    unf2(add2(w, f2(-b2.x, -b2.y)), u, v);
-                    lo = pack_h2(u, v);
-                }
+                const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                unf2(add2(w, f2(-b2.x, -b2.y)), u, v);
+                lo = pack_h2(u, v);
             };
             if (plain) {
                 const int e = max(of.z, of.w);
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                                 part(mul2(p, f2(g.z, g.w)), hi[2 * k + 1], lo[2 * k + 1]);
                             }
                             tmem_st_x8(sbuf + 32 * c + 8 * q, hi);
-                            if (PARTS == 2) tmem_st_x8(sbuf + 32 * c + 16 + 8 * q, lo);
+                            tmem_st_x8(sbuf + 32 * c + 16 + 8 * q, lo);
                         }
                         unf2(add2(sum0, sum1), u, v);
                         sum = __fadd_rn(u, v);
@@ -824,9 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                     }
                     const uint32_t to = sbuf + 32 * (c >> 1) + 8 * (c & 1);
                     // the chunk's second 16 scores lie where its small parts go: they are kept until those are read
-                    if (PARTS == 1) {
-                        tmem_st_x8(to, hi);
-                    } else if (c & 1) {
+                    if (c & 1) {
                         tmem_st_x8(to, hi);
                         tmem_st_x8(to + 16, lo);
                         tmem_st_x8(to + 8, keep);

@@ -1,0 +1,106 @@
+"""The key/value cache attention against tighter bounds than test_kv.py's, whose `2 n u max |v|` grows with the keys while the
+outputs shrink: here every weight has its own error and sums count their real depth, so that a probability held in too few
+bits, a key left out or a key taken twice shows at any length.
+
+u = 2^-24. A weight p_j = 2^(s_j - m) of a row carries
+  e_j = (2^-22 + (t + 8) u) S_j + 8 u |s_j| + 2^-33 max |q| K_j,   S_j = |scale| sum |q_d k_jd|,   K_j = |scale| sum of |k_jd| where q_d is not 0,
+for scores of t products (two fp16 parts of q: 2^-22 of the element or 2^-33 of the row's largest; fp32 sums; the factors'
+roundings), 2 u (|s_j - s_max| + 8) / ln 2 for the argument of the exponential, 2^-21 for the exponential, 2^-22 for the
+weight's own two parts. Those parts end at 2^-33 of the row's largest weight times its largest value scale (2^-32 next to a
+reference that is a whole number above the largest score). Sums of n keys: products are added 16 at a time for each of the
+two parts, each addition within 2^-23 (the tensor cores may cut off), 16 + n / 8 of them; the denominator 32 + n / 16 in u.
+  |err| <= sum p_j |v_j| (e_j + D_N) + |o| (sum p_j e_j + D_D + 4 u) + 2^-32 sum_j max p * max vs * |code_j|
+An output is then one rounding of what lies within that: o is between the rounded ends of the interval.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from b2s import kv  # noqa: E402
+from test_kv import BF16, E4M3, F32, I8, INVALID, TOP, U, UNSUPPORTED, Case, P, batch_struct, cache_struct, gen, gpu, ok, randn  # noqa: E402
+
+
+def interval(c, products):
+    """The ends of rows [0, c.rows) of the outputs in c's type, for scores of `products` nonzero products."""
+    cache, G = c.cache, c.heads // c.hkv
+    lo = torch.zeros(c.rows, c.heads, c.hd, dtype=torch.float64, device="cuda")
+    hi = torch.zeros_like(lo)
+    at = 0
+    for b, (n, L) in enumerate(zip(c.new, c.keys)):
+        def tokens(x):
+            x = x.float().double()
+            own = x[c.pages[b, :-(-L // cache.page_size)].long()].transpose(1, 2).reshape(-1, c.hkv, *x.shape[3:])[:L]
+            if c.prefix:
+                own = torch.cat((x[c.prefix_pages.long()].transpose(1, 2).reshape(-1, c.hkv, *x.shape[3:])[:c.prefix], own))
+            return own
+        k = tokens(cache.k) * tokens(cache.k_scale)[..., None]
+        vc, vs = tokens(cache.v), tokens(cache.v_scale)
+        q = c.q[at:at + n].double().view(n, c.hkv, G, c.hd)
+        N = k.shape[0]
+        last = L - n + torch.arange(n, device="cuda") if c.causal else torch.full((n,), L - 1, device="cuda")
+        seen = (torch.arange(N, device="cuda") <= c.prefix + last.clamp_min(-1)[:, None])[:, None].expand(n, G, N)
+        any_seen = seen.any(-1, keepdim=True)
+        for h in range(c.hkv if n and N else 0):
+            s = torch.einsum("igd,jd->igj", q[:, h], k[:, h]) * c.scale
+            S = torch.einsum("igd,jd->igj", q[:, h].abs(), k[:, h].abs()) * abs(c.scale)
+            K = abs(c.scale) * q[:, h].abs().amax(-1)[..., None] * ((q[:, h] != 0).double() @ k[:, h].abs().T)
+            low = s.masked_fill(~seen, -math.inf)
+            top = torch.where(any_seen, low.amax(-1, keepdim=True), 0.0)
+            p = torch.where(seen, torch.exp(low - top), 0.0)
+            total = torch.where(any_seen, p.sum(-1, keepdim=True), 1.0)
+            p = p / total
+            # up to 32 rows on int8 codes take a query as integers of 24 bits under its largest element
+            low_q = U if cache.k.dtype == I8 and n * G <= 32 else 2.0 ** -33
+            e = (2.0 ** -22 + (products + 8) * U) * S + 8 * U * s.abs() + low_q * K
+            e = e + 2 * U * ((s - top).abs() + 8) / math.log(2) + 2.0 ** -21 + 2.0 ** -22
+            e = torch.where(seen, e, 0.0)
+            count = seen.sum(-1, keepdim=True).double()
+            v = vc[:, h] * vs[:, h][:, None]
+            o = p @ v
+            most = torch.where(seen, vs[:, h].abs(), 0.0).amax(-1, keepdim=True) / total
+            tol = (p * (e + (16 + count / 8) * 2.0 ** -23)) @ v.abs() + o.abs() * ((p * e).sum(-1, keepdim=True) + (36 + count / 16) * U)
+            tol = 1.01 * (tol + 2.0 ** -32 * most * (seen.double() @ vc[:, h].abs())) + 1e-37
+            tol = torch.where(any_seen, tol, 0.0)
+            lo[at:at + n, h * G:(h + 1) * G], hi[at:at + n, h * G:(h + 1) * G] = o - tol, o + tol
+        at += n
+    return [x.view(c.rows, -1).float().to(c.dtype) for x in (lo, hi)]
+
+
+def inside(c, o, products):
+    lo, hi = interval(c, products)
+    got = o[:c.rows]
+    out = ~((got >= lo) & (got <= hi))
+    where = out.nonzero()[0].tolist() if bool(out.any()) else None
+    assert where is None, (f"{int(out.sum())} of {out.numel()} outputs, the first at {where}: {float(got[tuple(where)])!r} is not in "
+                           f"[{float(lo[tuple(where)])!r}, {float(hi[tuple(where)])!r}]")
+    assert bool((o[c.rows:] == 7).all())
+
+
+def one_product(c, gain):
+    """Queries with one nonzero element a head, of about `gain`, so that a score is one product and as good as exact."""
+    g = gen(c.rows + c.heads)
+    at = torch.randint(0, c.hd, (c.rows, c.heads, 1), generator=g, device="cuda")
+    q = torch.zeros(c.rows, c.heads, c.hd, device="cuda")
+    q.scatter_(2, at, gain * randn(g, c.rows, c.heads, 1))
+    c.q = q.view(c.rows, -1).to(c.dtype)
+    return c
+
+
+MANY = [  # new, keys, heads, kv heads, hd, prefix: one row block and several, pairs of them (bf16), cut keys, both prefix forms
+    ([90], [300], 2, 2, 64, 0), ([70, 3, 260], [70, 90, 700], 8, 2, 128, 0), ([1100], [1100], 4, 1, 112, 0),
+    ([1] * 40, [30] * 40, 32, 8, 128, 1000), ([100, 1, 30], [120, 5, 30], 16, 4, 48, 300), ([1] * 9, [1, 15, 16, 17, 63, 64, 65, 700, 2], 20, 5, 128, 0)]
+
+
+@gpu
+@pytest.mark.parametrize("new,keys,heads,hkv,hd,prefix", MANY)
+@pytest.mark.parametrize("dtype,code", [(BF16, E4M3), (BF16, I8)])
+def test_outputs_are_one_rounding_of_the_exact_ones(b2s, new, keys, heads, hkv, hd, prefix, dtype, code):
+    """Sharp scores that are single products: weights of a few keys, each held to 2^-22 whatever the type of the rows."""
+    c = one_product(Case(3 + hd + sum(keys), new, keys, heads, hkv, hd, 16, dtype, code, True, prefix), 25.0)
+    o = c.run()
+    ok(b2s)
+    inside(c, o, 1)
