@@ -90,7 +90,8 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache *cache, const b2s_kv_b
  * tokens j <= kv_len - n + i, else all. A row that sees nothing is written as zeros; rows of o outside
  * [q_start[0], q_start[batch]) are left as they were. o may be q. scale is finite and below 2^127.
  * Scores, softmax and sums are fp32, products run on the tensor cores, where the 8-bit codes are exact. fp32 queries
- * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or 2^-40 of its row's largest one), or,
+ * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or of its row's largest one 2^-39 where few
+ * rows share a key/value head and 2^-32 for a probability where many do; its value scale is part of the element), or,
  * queries on int8 codes, as integers of 24 bits under the row's largest element; bf16 queries likewise or exactly, their
  * probabilities as fp32 ones. A query head with an infinity or a NaN is NaN; no other one is. */
 int b2s_attention_kv(const b2s_kv_cache *cache, const b2s_kv_batch *batch, int32_t type, const void *q, int64_t ldq,

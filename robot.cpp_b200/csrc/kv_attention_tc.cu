@@ -21,15 +21,17 @@
 // chain a group the tensor cores and the exponentials waited for each other (a pair of tiles took 7500 clocks, of which the
 // products are 2048 and the exponentials 2048). Sixteen warps also because one warp a scheduler needs 570 clocks for 32 keys'
 // exponentials and four need 280 each (measured alone; the special-function unit's own limit is 256).
-// The reference of the exponentials is a whole number that moves only when probabilities grow past 2^8: sums, outputs and
+// The reference of the exponentials is a whole number that moves only when probabilities grow past 2^5: sums, outputs and
 // probabilities are then multiplied by a power of two, which is exact. So scores are read once and no maximum is formed: 32
-// probabilities whose sum is at most 2^8 are each at most that, and only a larger sum asks for their maximum. A row's
+// probabilities whose sum is at most 2^5, which those at or below their reference never pass, are each at most that, and only a
+// larger sum asks for their maximum. (With 2^8 the references move less, and fp32 chunks took 183 us for the 192 below, but
+// probabilities have four bits fewer above the end of fp16.) A row's
 // outputs have one reference; its two streams commit their products to it in turn, and whoever finds the other's reference
 // changed brings its own probabilities, or the outputs, under the larger one.
 //
 // Measured: 2 x up to 2048 bf16 tokens on 8192 e4m3 ones, causal, 32 heads on 8 of 128: 722 us, 492 TFLOP/s of the 1640 that a
-// library product reaches (738 with P's second part counted); 1024 tokens on 4096 with 20 heads on 5: 149 us (fp32, whose Q has
-// two parts too, 183 us). A stream's chain for 64 keys bounds it, no unit does, and tensor memory has no columns for more streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the
+// library product reaches (738 with P's second part counted); 1024 tokens on 4096 with 20 heads on 5: 151 us (fp32, whose Q has
+// two parts too, 192 us). A stream's chain for 64 keys bounds it, no unit does, and tensor memory has no columns for more streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the
 // first codes) and end (6,000): 8 prompts of 288 fp32 tokens take 58 us.
 //
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             for (auto& v : x) v = __float_as_uint(__fmul_rn(__fmul_rn(__uint_as_float(v), f0), f1));
         };
         float m = -INFINITY, l = 0.0f;  // reference and sum of this thread's keys
-        int vref = 8;
+        int vref = 12;
         // ---- this stream's MMAs, issued by one of its warps: another scheduler's for each stream
         const bool leader = quad == st;
         const uint32_t q0 = smem_u32(sQ) + (PAIR ? wg * kTileBytes : 0), s0 = tmem + st * kHalf, o0 = tmem + kOcol + wg * kRows;
@@ -709,13 +711,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 const int e = max(of.z, of.w);
                 if (e >= vref) vref = min(e + 2, 255);
                 // P of 32 keys over their scores: p = 2^(s - m + shift) times the value scales, which are over 2^(exponent + 1)
-                // of their 32 keys (one far below the reference counts as 2^-60); their sum is taken back by 2^-shift
+                // of their 32 keys (one far below the reference counts as 2^-60); their sum is taken back by 2^-shift. With
+                // shift = 9, or 10 where the exponent has grown by one, P stays below 2^15, and its small parts, which end at
+                // 2^-24, round the row's largest product of probability and value scale at 2^-33 of it (2^-32 where its score
+                // is a unit below the reference)
 #pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
                     const float4* ksp = reinterpret_cast<const float4*>(&ms->ks[sc][half * kHalf + 32 * c]);
                     const float4* vnp = reinterpret_cast<const float4*>(&ms->vn[sc][half * kHalf + 32 * c]);
-                    const int shift = max(-60, ms->of[sc][half].vexp[c] + 7 - vref);
-                    const float most = pow2_biased(127 + 8 + shift);
+                    const int shift = max(-60, ms->of[sc][half].vexp[c] + 11 - vref);
+                    const float most = pow2_biased(127 + 5 + shift);
                     uint32_t x[32];
                     float sum;
                     tmem_ld_32x32b_x32(sbuf + 32 * c, x);
@@ -756,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                             mx = max3(mx, __fmul_rn(__uint_as_float(x[4 * k + 2]), f.z), __fmul_rn(__uint_as_float(x[4 * k + 3]), f.w));
                         }
                         float f = 1.0f;
-                        if (mx > __fadd_rn(m, 8.0f)) {
+                        if (mx > m) {
                             const float mn = ceilf(mx);
                             f = down(m, mn);
                             l = __fmul_rn(l, f);
@@ -789,12 +794,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 }
                 const int e = __float_as_int(vmx) >> 23;
                 if (e >= vref) vref = min(e + 2, 255);
-                if (mx > __fadd_rn(m, 8.0f)) {
+                if (mx > __fadd_rn(m, 5.0f)) {
                     const float mn = ceilf(mx);
                     l = __fmul_rn(l, down(m, mn));
                     m = mn;
                 }
-                const float mu = m == -INFINITY ? 0.0f : -m, vmul = pow2_biased(260 - vref);
+                const float mu = m == -INFINITY ? 0.0f : -m, vmul = pow2_biased(264 - vref);
                 uint32_t keep[8];
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
@@ -839,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             // ---- one reference for the row's outputs: the other stream has left the one that its last half tile went in with
             if (i + half > 0) wait(ms, &ms->mpost[st ^ 1], (uint32_t)(half ? i : i - 1) & 1u);
             const float mo = i + half > 0 ? ms->om[wg][r] : -INFINITY;
-            const int vo = i + half > 0 ? ms->ov[wg][r] : 8;
+            const int vo = i + half > 0 ? ms->ov[wg][r] : 12;
             if (__any_sync(0xffffffffu, m != mo || vref != vo)) {
                 const float mn = fmaxf(m, mo);
                 const int vn = max(vref, vo);
@@ -886,7 +891,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         // ---- results: half of the columns of its row for each thread, a quarter where both groups have the same rows
         if (n == 0) {
             ms->om[wg][r] = -INFINITY;
-            ms->ov[wg][r] = 8;
+            ms->ov[wg][r] = 12;
         } else {
             wait(ms, &ms->mpost[st | 1], (uint32_t)(n - 1) & 1u);
             const float mf = ms->om[wg][r];  // the last reference
@@ -896,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         tc_fence_before();
         asm volatile("bar.sync 1, 512;" ::: "memory");  // every product has been made: Q and K are not read any more
         tc_fence_after();
-        float f0 = pow2_biased(ms->ov[wg][r] - 6), f1 = 0.0f;
+        float f0 = pow2_biased(ms->ov[wg][r] - 10), f1 = 0.0f;
         m = ms->om[wg][r];
         l = __fadd_rn(ms->l[wg][0][r], ms->l[wg][1][r]);
         if (!PAIR) {
@@ -904,8 +909,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             m = fmaxf(ma, mb);
             const float fa = ma == -INFINITY ? 0.0f : ex2(__fsub_rn(ma, m)), fb = mb == -INFINITY ? 0.0f : ex2(__fsub_rn(mb, m));
             l = __fmaf_rn(__fadd_rn(ms->l[0][0][r], ms->l[0][1][r]), fa, __fmul_rn(__fadd_rn(ms->l[1][0][r], ms->l[1][1][r]), fb));
-            f0 = __fmul_rn(pow2_biased(ms->ov[0][r] - 6), fa);
-            f1 = __fmul_rn(pow2_biased(ms->ov[1][r] - 6), fb);
+            f0 = __fmul_rn(pow2_biased(ms->ov[0][r] - 10), fa);
+            f1 = __fmul_rn(pow2_biased(ms->ov[1][r] - 10), fb);
         }
         const int c0 = PAIR ? half * (HDP / 2) : (2 * wg + half) * (HDP / 4), c1 = c0 + (PAIR ? HDP / 2 : HDP / 4);
         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);

@@ -104,3 +104,26 @@ def test_outputs_are_one_rounding_of_the_exact_ones(b2s, new, keys, heads, hkv, 
     o = c.run()
     ok(b2s)
     inside(c, o, 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [8, 96, 300])
+@pytest.mark.parametrize("down", [13.0, 18.0, 21.0])
+def test_weights_far_below_the_largest_keep_their_bits(b2s, dtype, rows, down):
+    """One token of value zero has all but 2^-down .. 2^-(down + 2) of each weight of the others: they alone make the output, and all
+    are rounded alike, so that errors add up."""
+    c = Case(113, [rows], [120], 1, 1, 64, 16, dtype, I8, False, scale=1.0)
+    c.cache.k.zero_()
+    c.cache.k_scale.fill_(1.0)
+    c.cache.v.fill_(100)
+    c.cache.v_scale.fill_(0.013)
+    page = int(c.pages[0, 0])
+    c.cache.k[page, :, 0, 5] = 16
+    c.cache.v[page, :, 0] = 0
+    c.q = torch.zeros(rows, 64, device="cuda")
+    c.q[:, 5] = (down + torch.arange(rows, device="cuda") * (2.0 / rows)) * math.log(2) / 16
+    c.q = c.q.to(dtype)
+    o = c.run()
+    ok(b2s)
+    inside(c, o, 1)
