@@ -5,7 +5,7 @@
 // (bf16) or two (fp32) fp16 parts, and the probabilities times the value scale are two. One MMA a part:
 //   S = sum over parts Q_part K^T,  O += sum over parts P_part V   (fp32 accumulation in tensor memory).
 // One part of P would round each weight to 2^-11: 2 to 5% of bf16 outputs then came out a step off (a chunk of 2048 tokens on
-// 8192 took 572 us with it and takes 722 with two).
+// 8192 took 572 us with it and takes 702 with two).
 // Floor: 2 * pairs * hd operations a head for each part of Q and P, at the fp16 rate; next to it the exponentials, 16 a clock
 // and SM.
 //
@@ -21,18 +21,19 @@
 // chain a group the tensor cores and the exponentials waited for each other (a pair of tiles took 7500 clocks, of which the
 // products are 2048 and the exponentials 2048). Sixteen warps also because one warp a scheduler needs 570 clocks for 32 keys'
 // exponentials and four need 280 each (measured alone; the special-function unit's own limit is 256).
-// The reference of the exponentials is a whole number that moves only when probabilities grow past 2^5: sums, outputs and
-// probabilities are then multiplied by a power of two, which is exact. So scores are read once and no maximum is formed: 32
-// probabilities whose sum is at most 2^5, which those at or below their reference never pass, are each at most that, and only a
-// larger sum asks for their maximum. (With 2^8 the references move less, and fp32 chunks took 183 us for the 192 below, but
-// probabilities have four bits fewer above the end of fp16.) A row's
-// outputs have one reference; its two streams commit their products to it in turn, and whoever finds the other's reference
-// changed brings its own probabilities, or the outputs, under the larger one.
+// The reference of the exponentials is a whole number that moves only when probabilities grow past 2^5: sums and outputs are
+// then multiplied by a power of two, which is exact, and the half tile's probabilities too, which keep what their two parts can
+// hold. So scores are read once and no maximum is formed: 32 probabilities whose sum is at most 2^5, which those at or below
+// their reference never pass, are each at most that, and only a larger sum asks for their maximum. (With 2^8 the references
+// move less and fp32 chunks took 4% less time, but probabilities have four bits fewer above the end of fp16.) A row's outputs
+// have one reference; its two streams commit their products to it in turn, and whoever finds the other's reference changed
+// brings its own probabilities, or the outputs, under the larger one.
 //
-// Measured: 2 x up to 2048 bf16 tokens on 8192 e4m3 ones, causal, 32 heads on 8 of 128: 722 us, 492 TFLOP/s of the 1640 that a
-// library product reaches (738 with P's second part counted); 1024 tokens on 4096 with 20 heads on 5: 151 us (fp32, whose Q has
-// two parts too, 192 us). A stream's chain for 64 keys bounds it, no unit does, and tensor memory has no columns for more streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the
-// first codes) and end (6,000): 8 prompts of 288 fp32 tokens take 58 us.
+// Measured: 2 x up to 2048 bf16 tokens on 8192 e4m3 ones, causal, 32 heads on 8 of 128: 702 us, 506 TFLOP/s of the 1640 that a
+// library product reaches (759 with P's second part counted); 1024 tokens on 4096 with 20 heads on 5: 148 us (fp32, whose Q has
+// two parts too, 197 us). A stream's chain for 64 keys bounds it, no unit does, and tensor memory has no columns for more
+// streams. A block of few tiles is mostly start (10,000 clocks: lengths, pages, Q, the first codes) and end (6,000): 8 prompts of
+// 288 fp32 tokens take 59 us.
 //
 // Every wait is bounded: after one that ran out the error word is set, further waits of the block return at once, no more
 // MMAs are issued, those in flight are waited for, and tensor memory is freed.
@@ -190,6 +191,19 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
     asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) : : "memory");
 }
 
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[8], uint32_t (&s)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(s[0]),
+                   "+r"(s[1]), "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -678,22 +692,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
             };
             wait(ms, &ms->sfull[st], (uint32_t)i & 1u);
             tc_fence_after();
-            auto scale_probabilities = [&](int chunks, float f) {  // the half tile's first chunks of 32 keys
-                tc_wait_st();
-                const __half2 f2h = __float2half2_rn(f);
-#pragma unroll 1
-                for (int c = 0; c < 32 * chunks; c += 16) {
-                    uint32_t x[16];
-                    tmem_ld_x16(sbuf + c, x);
-                    wait_ld(x);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&x[k]), f2h);
-                        x[k] = *reinterpret_cast<const uint32_t*>(&z);
-                    }
-                    tmem_st_x16(sbuf + c, x);
-                }
-            };
             // 2^(from - to) for whole numbers from <= to; 0 from -inf
             auto down = [&](float from, float to) {
                 const float by = __fsub_rn(from, to);
@@ -706,6 +704,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
                 const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
                 unf2(add2(w, f2(-b2.x, -b2.y)), u, v);
                 lo = pack_h2(u, v);
+            };
+            // The half tile's first chunks of 32 keys. The parts are put together, multiplied and split anew: an fp16 factor ends at
+            // 2^-24, where a jump of the scores or of the value scales does not, and parts scaled by themselves lose their low bits.
+            auto scale_probabilities = [&](int chunks, float f) {
+                tc_wait_st();
+#pragma unroll 1
+                for (int c = 0; c < 2 * chunks; ++c) {
+                    const uint32_t at = sbuf + 32 * (c >> 1) + 8 * (c & 1);
+                    uint32_t hi[8], lo[8];
+                    tmem_ld_x8(at, hi);
+                    tmem_ld_x8(at + 16, lo);
+                    wait_ld(hi, lo);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&lo[k]));
+                        part(mul2(add2(f2(h.x, h.y), f2(g.x, g.y)), f2(f, f)), hi[k], lo[k]);
+                    }
+                    tmem_st_x8(at, hi);
+                    tmem_st_x8(at + 16, lo);
+                }
             };
             if (plain) {
                 const int e = max(of.z, of.w);

@@ -97,7 +97,7 @@ MANY = [  # new, keys, heads, kv heads, hd, prefix: one row block and several, p
 
 @gpu
 @pytest.mark.parametrize("new,keys,heads,hkv,hd,prefix", MANY)
-@pytest.mark.parametrize("dtype,code", [(BF16, E4M3), (BF16, I8)])
+@pytest.mark.parametrize("dtype,code", [(BF16, E4M3), (BF16, I8), (F32, I8), (F32, E4M3)])
 def test_outputs_are_one_rounding_of_the_exact_ones(b2s, new, keys, heads, hkv, hd, prefix, dtype, code):
     """Sharp scores that are single products: weights of a few keys, each held to 2^-22 whatever the type of the rows."""
     c = one_product(Case(3 + hd + sum(keys), new, keys, heads, hkv, hd, 16, dtype, code, True, prefix), 25.0)
@@ -127,3 +127,31 @@ def test_weights_far_below_the_largest_keep_their_bits(b2s, dtype, rows, down):
     o = c.run()
     ok(b2s)
     inside(c, o, 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [8, 64, 300])
+@pytest.mark.parametrize("what", ["score", "value scale"])
+def test_a_jump_along_the_keys_leaves_the_earlier_ones_their_weight(b2s, dtype, rows, what):
+    """One token of value zero whose score lies 24 to 29 powers of two above the others', or whose value scale does: wherever it
+    stands in a tile, the weights before it are taken under its reference, none is lost."""
+    for at in (33, 40, 64, 95, 127, 128, 200, 330):
+        for jump in (24, 27, 29):
+            c = Case(117, [rows], [340], 1, 1, 64, 16, dtype, I8, False, scale=1.0)
+            c.cache.k.zero_()
+            c.cache.k_scale.fill_(1.0)
+            c.cache.v.fill_(100)
+            c.cache.v_scale.fill_(1.0)
+            page, off = int(c.pages[0, at // 16]), at % 16
+            c.cache.v[page, :, off] = 0
+            c.q = torch.zeros(rows, 64, device="cuda")
+            if what == "score":
+                c.cache.k[page, :, off, 5] = 16
+                c.q[:, 5] = jump * math.log(2) / 16
+            else:
+                c.cache.v_scale[page, :, off] = 2.0 ** jump
+            c.q = c.q.to(dtype)
+            o = c.run()
+            ok(b2s)
+            inside(c, o, 1)
