@@ -390,12 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
         return min(253, 268 - (__float_as_int(big) >> 23));
     };
 
-    // A row far below it has its own, so that it keeps its bits beside a huge one (fp16 parts end at 2^-24); its scores are
-    // brought level where they are read.
+    // A row further below it than 2^6 has its own, and its scores are brought level where they are read, off the fast path. The
+    // others keep the block's: fp16 parts end at 2^-24 and round at 2^-25, which is 2^-33 of such a row's largest element.
     auto up_of_row = [&](int common, int row) {
         const uint32_t bits = ms->row_big[row];
         const int own = min(253, 268 - (int)(bits >> 23));
-        return bits == 0 || own - common <= 12 ? common : own;
+        return bits == 0 || own - common <= 6 ? common : own;
     };
 
     if (warp >= kSoftWarps) {

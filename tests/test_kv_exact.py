@@ -155,3 +155,28 @@ def test_a_jump_along_the_keys_leaves_the_earlier_ones_their_weight(b2s, dtype, 
             o = c.run()
             ok(b2s)
             inside(c, o, 1)
+
+
+@gpu
+@pytest.mark.parametrize("code", [I8, E4M3])
+@pytest.mark.parametrize("rows", [6, 64, 200])
+def test_a_query_row_keeps_its_bits_beside_a_larger_one(b2s, code, rows):
+    """Rows 2^0 to 2^13 below the block's largest whose scores come from elements 2^-20 of their own largest one: even keys look at
+    one of them, odd keys at another, so that the elements' own errors part their weights."""
+    c = Case(121, [rows], [200], 2, 1, 64, 16, F32, code, False, scale=2.0 ** 21)
+    k, v = torch.zeros(200, 64, device="cuda"), torch.full((200, 64), 96.0, device="cuda")
+    k[0::2, 7], k[1::2, 8], v[1::2] = 96.0, 96.0, -96.0
+    j = torch.arange(200, device="cuda")
+    for to, x in ((c.cache.k, k), (c.cache.v, v)):
+        to.view(torch.uint8)[c.pages[0, j // 16].long(), 0, j % 16] = x.to(code).view(torch.uint8)
+    for t in (c.cache.k_scale, c.cache.v_scale):
+        t.fill_(0.01)
+    g = gen(122)
+    q = torch.zeros(rows, 2, 64, device="cuda")
+    q[:, :, 3] = 1.0 + torch.rand((rows, 2), generator=g, device="cuda")
+    q[:, :, 7:9] = (1.0 + 0.1 * torch.rand((rows, 2, 2), generator=g, device="cuda")) * 2.0 ** -20
+    by = torch.pow(2.0, (torch.arange(rows, device="cuda") % 14).float())
+    c.q = (q * by[:, None, None]).view(rows, -1)
+    o = c.run()
+    ok(b2s)
+    inside(c, o, 3)
