@@ -101,7 +101,8 @@ int b2s_attention_kv(const b2s_kv_cache *cache, const b2s_kv_batch *batch, int32
 /* The same with prefix_len tokens in front of every sequence that all of them share: token j of the prefix is in page
  * prefix_pages[j / page_size] (device, ceil(prefix_len / page_size) entries). kv_len counts the sequence's own tokens
  * behind it; every query row sees the whole prefix. The prefix is read once for the batch and joined with the own
- * tokens by the two parts' maxima and sums. prefix_len = 0 is b2s_attention_kv. */
+ * tokens by the two parts' maxima and sums. (A short prefix is read by each sequence instead, where that takes less time.)
+ * Where q_start[batch] is below a sequence's rows, that sequence may be left out too. prefix_len = 0 is b2s_attention_kv. */
 int b2s_attention_kv_prefix(const b2s_kv_cache *cache, const b2s_kv_batch *batch, const int32_t *prefix_pages,
                             int64_t prefix_len, int32_t type, const void *q, int64_t ldq, int64_t M, int n_heads,
                             float scale, int causal, void *o, int64_t ldo, void *workspace, size_t workspace_bytes,

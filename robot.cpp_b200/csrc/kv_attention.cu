@@ -151,7 +151,7 @@ __device__ __forceinline__ Seq seq_of(const KvAttnArgs& a, int b) {
     const int lo = a.q_start[b * a.q_stride], hi = a.q_start[(b + 1) * a.q_stride];
     int64_t len = a.kv_len ? (int64_t)a.kv_len[b] : a.kv_const;
     const int64_t cap = a.max_pages << a.c.page_shift;
-    bool bad = lo < 0 || hi < lo || hi > a.M;
+    bool bad = lo < 0 || hi < lo || hi > a.M || (a.add.pieces > 0 && hi > rows_used(a, a.q_start[a.batch]));
     s.lo = lo;
     s.n = bad ? 0 : hi - lo;
     if (len < 0 || len > cap) {

@@ -248,7 +248,11 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
 
 __device__ __forceinline__ Rows rows_of(const KvAttnArgs& a, int b) {
     Rows s;
-    const int lo = a.q_start[b * a.q_stride], hi = a.q_start[(b + 1) * a.q_stride];
+    int lo = a.q_start[b * a.q_stride], hi = a.q_start[(b + 1) * a.q_stride];
+    if (!a.kv_len) {  // a shared prefix: every row that a sequence in range can have gets its state
+        lo = 0;
+        hi = rows_used(a, hi);
+    }
     int64_t len = a.kv_len ? (int64_t)a.kv_len[b] : a.kv_const;
     const int64_t cap = a.max_pages << a.c.page_shift;
     bool bad = lo < 0 || hi < lo || hi > a.M;
@@ -1036,6 +1040,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_state_join_kernel(const KvAtt
         if (lo < 0) continue;
         const Rows sq = rows_of(a, lo);
         if (sq.rows == 0 || row >= sq.lo + (int64_t)sq.n) continue;
+        if (a.add.pieces > 0 && sq.lo + sq.n > rows_used(a, a.q_start[a.batch])) continue;  // no state from the prefix
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         const int pieces = a.out.pieces + a.add.pieces;

@@ -71,6 +71,10 @@ struct KvAttnArgs {
     int prefix_len, prefix_pad;     // prefix_pad: in whole tiles
 };
 
+// The rows that a pass over a shared prefix takes, from 0 on: up to the batch's last entry of q_start, or, where that is out of
+// range, all. Sequences that reach past it find no state there and are left out.
+__device__ __forceinline__ int rows_used(const KvAttnArgs& a, int end) { return end < 0 || end > a.M ? (int)a.M : end; }
+
 // Few rows (kv_attention.cu).
 size_t kv_attn_part_bytes();
 cudaError_t launch_kv_attention(const KvAttnArgs& a, cudaStream_t st);

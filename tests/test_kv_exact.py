@@ -180,3 +180,28 @@ def test_a_query_row_keeps_its_bits_beside_a_larger_one(b2s, code, rows):
     o = c.run()
     ok(b2s)
     inside(c, o, 3)
+
+
+@gpu
+@pytest.mark.parametrize("new,prefix", [([1] * 70, 600), ([80, 1, 70], 300), ([3, 120, 2, 90], 5000)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_bad_row_range_behind_a_prefix_touches_no_other_sequence(b2s, new, prefix, dtype):
+    """The prefix as a pass of its own over all rows: a sequence whose range is out of order is left out, the others see the
+    prefix all the same. A last entry below their rows leaves them out, rather than without a prefix."""
+    keys = [5 + 7 * (i % 9) + (x if x > 4 else 0) for i, x in enumerate(new)]
+    c = Case(131, new, keys, 32, 8, 64, 16, dtype, I8, True, prefix, extra_rows=4)
+    start = c.q_start.clone()
+    ref, tol = c.reference()
+    first, last = new[0], c.rows - new[-1]
+    second = int(start[2])
+    for at, value, good in ((0, -1, slice(first, c.rows)), (0, first + 1, slice(first, c.rows)), (0, 2 ** 31 - 1, slice(first, c.rows)),
+                            (1, -5, slice(second, c.rows)), (len(new), c.rows + 5, slice(0, last)), (len(new), -2 ** 31, slice(0, last)),
+                            (len(new), 0, slice(0, 0))):
+        c.q_start.copy_(start)
+        c.q_start[at] = value
+        o = c.run()
+        ok(b2s, 4)
+        assert bool(((o[:c.rows].double() - ref).abs() <= tol)[good].all())
+        rest = torch.ones(o.shape[0], dtype=torch.bool, device="cuda")
+        rest[good] = False
+        assert bool((o[rest] == 7).all())
