@@ -1037,9 +1037,21 @@ __global__ void __launch_bounds__(kJoinThreads) kv_state_join_kernel(const KvAtt
                 if (step == 1) break;
             }
         }
-        if (lo < 0) continue;
+        auto has = [&](int b) {
+            const int first = a.q_start[b], end = a.q_start[b + 1];
+            return first >= 0 && first <= row && row < end && end <= a.M;
+        };
+        if (lo < 0 || !has(lo)) {
+            // behind the last sequence, or an entry out of order has led the search astray
+            if (lo == a.batch - 1 && a.q_start[lo] >= 0) continue;
+            int found = a.batch;
+            for (int b = lane; b < a.batch && found == a.batch; b += 32)
+                if (has(b)) found = b;
+            lo = __reduce_min_sync(0xffffffffu, found);
+            if (lo == a.batch) continue;
+        }
         const Rows sq = rows_of(a, lo);
-        if (sq.rows == 0 || row >= sq.lo + (int64_t)sq.n) continue;
+        if (sq.rows == 0) continue;
         if (a.add.pieces > 0 && sq.lo + sq.n > rows_used(a, a.q_start[a.batch])) continue;  // no state from the prefix
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

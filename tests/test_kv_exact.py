@@ -205,3 +205,23 @@ def test_a_bad_row_range_behind_a_prefix_touches_no_other_sequence(b2s, new, pre
         rest = torch.ones(o.shape[0], dtype=torch.bool, device="cuda")
         rest[good] = False
         assert bool((o[rest] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("prefix", [0, 300])
+def test_a_bad_row_range_in_the_middle_touches_no_sequence_before_it(b2s, prefix):
+    """Rows whose pieces are joined find their sequence although an entry of q_start behind theirs is out of order."""
+    new = [80, 40, 60, 2]
+    c = Case(133, new, [400, 300, 200, 9], 8, 2, 64, 16, F32, I8, True, prefix, extra_rows=4)
+    start = c.q_start.clone()
+    ref, tol = c.reference()
+    for at in (1, 2, 3):
+        for value in (-5, 2 ** 31 - 1):
+            c.q_start.copy_(start)
+            c.q_start[at] = value
+            o = c.run()
+            ok(b2s, 4)
+            good = torch.ones(c.rows, dtype=torch.bool, device="cuda")
+            good[int(start[at - 1]):int(start[at + 1])] = False
+            assert bool(((o[:c.rows].double() - ref).abs() <= tol)[good].all())
+            assert bool((o[:c.rows][~good] == 7).all() and (o[c.rows:] == 7).all())
