@@ -80,8 +80,9 @@ int b2s_kv_write(const b2s_kv_cache *cache, int32_t type, const void *k, int64_t
 int b2s_kv_read(const b2s_kv_cache *cache, const int64_t *slots, int64_t M, int32_t type, void *k, int64_t ldk, void *v,
                 int64_t ldv, void *stream);
 
-/* Workspace bytes of the attention calls for these shapes (M = rows of q; prefix_len = 0 for b2s_attention_kv); 0 if
- * they are not valid. It is scratch of one call: nothing is kept in it, and calls that may overlap need one each. */
+/* Workspace bytes of the attention calls for these shapes (M = rows of q; prefix_len = 0 for b2s_attention_kv) and for
+ * calls on the same cache and n_heads whose M, batch, max_q, max_pages and prefix_len are no larger; 0 if they are not
+ * valid. It is scratch of one call: nothing is kept in it, and calls that may overlap need one each. */
 size_t b2s_attention_kv_workspace_size(const b2s_kv_cache *cache, const b2s_kv_batch *batch, int64_t M, int n_heads,
                                        int64_t prefix_len);
 

@@ -90,21 +90,61 @@ struct Plan {
 // join. bf16, five heads, us with blocks of 128 and of 256 rows: one sequence of 256 rows on 2000 keys 19 and 27, 8 of 260 on
 // 2000 keys 45 and 76, 2 of 2048 on 4096 keys 144 and 119, 8 of 512 on 128 keys 23 and 18. fp32, whole keys and cut ones: 260
 // rows on 8192 keys 175 and 40, 512 on 2000 keys 54 and 27, 4096 rows of one head on 4096 keys 94 and 41.
+constexpr int kMaxSplits = 16, kWave = 148;
+// Numbers of tiles that are planned for: each up to 64, then eight an octave, so that most_pieces can go through them all.
+int64_t tile_step(int64_t tiles) {
+    int64_t step = 1;
+    while (tiles / step >= (step == 1 ? 64 : 16)) step *= step == 1 ? 8 : 2;
+    return step;
+}
+int64_t planned_tiles(int64_t keys) {
+    const int64_t tiles = std::max<int64_t>(1, (keys + 127) / 128), step = tile_step(tiles);
+    return (tiles + step - 1) / step * step;
+}
+// The number of shares of the least estimate for `units` blocks' worth of whole rows, and that estimate.
+int best_splits(int64_t units, int64_t tiles, int pair, int64_t* least) {
+    int best = 1;
+    for (int s = 1; s <= kMaxSplits && s <= tiles && (s == 1 || units < kWave); ++s) {
+        const int64_t cost = (units * s + kWave - 1) / kWave * ((tiles + s - 1) / s * (2 + pair) + 8 + 4 * pair) + (s > 1 ? 6 : 0);
+        if (s == 1 || cost < *least) {
+            *least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
 void plan_blocks(Plan* p, int64_t M, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
     p->many = true;
-    const int64_t seqs = (M + max_q - 1) / max_q, tiles = std::max<int64_t>(1, (keys + 127) / 128);
+    const int64_t seqs = std::max<int64_t>(1, (M + max_q - 1) / max_q), tiles = planned_tiles(keys);
     int64_t best = -1;
     for (int pair = 0; pair <= (bf16 ? 1 : 0); ++pair) {
-        const int64_t units = std::max<int64_t>(1, seqs) * ((max_q * group + 128 * (1 + pair) - 1) / (128 * (1 + pair))) * kv_heads;
-        for (int s = 1; s <= 16 && s <= tiles && (s == 1 || units < 148); ++s) {
-            const int64_t cost = (units * s + 147) / 148 * ((tiles + s - 1) / s * (2 + pair) + 8 + 4 * pair) + (s > 1 ? 6 : 0);
-            if (best < 0 || cost < best) {
-                best = cost;
-                p->pair = pair != 0;
-                p->splits = s;
+        int64_t cost = 0;
+        const int s = best_splits(seqs * ((max_q * group + 128 * (1 + pair) - 1) / (128 * (1 + pair))) * kv_heads, tiles, pair, &cost);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p->pair = pair != 0;
+            p->splits = s;
+        }
+    }
+}
+// The most pieces (of a row and head) that cut keys leave in any call of up to `rows` rows x heads over up to `keys` keys: calls of
+// fewer rows or keys may be cut where the largest is not. M rows in blocks of 128 or 256 a sequence and key/value head are at most
+// that many rows x heads for each unit.
+int64_t most_pieces(int64_t rows, int kv_heads, int64_t keys) {
+    int64_t most = 0;
+    const int64_t last = planned_tiles(keys);
+    for (int64_t units = (kWave - 1) / kv_heads * kv_heads; units > 0; units -= kv_heads) {
+        for (int pair = 0; pair < 2; ++pair) {
+            const int64_t held = std::min(rows, units * 128 * (1 + pair));
+            if (held * kMaxSplits <= most) continue;
+            for (int64_t tiles = 2; tiles <= last; tiles += tile_step(tiles)) {
+                int64_t cost = 0;
+                const int s = best_splits(units, tiles, pair, &cost);
+                if (s > 1) most = std::max(most, held * s);
             }
         }
     }
+    return most;
 }
 Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
     Plan p{true, false, false, 0, 1};
@@ -121,10 +161,13 @@ Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads,
 // place of three. 20 heads on 5, int8, us with one pass and with three: 16 rows on 545 shared tokens (1440 steps) 21.5 and 25.1,
 // 32 on 1600 (8000) 30.2 and 31.0, 64 on 800 (8000) 32.4 and 30.2, 64 on 1600 (16000) 43.9 and 32.4.
 constexpr int64_t kPrefixSteps = 8192;
+bool prefix_inline(bool own_many, int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t prefix_len) {
+    return M == 0 || (!own_many && batch * kv_heads * ((std::min(max_q, M) * group + 7) / 8) * ((prefix_len + 31) / 32) <= kPrefixSteps);
+}
 Plan plan_prefix(const Plan& own, int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t prefix_len, bool bf16) {
     Plan p{false, false, false, 0, 1};
     if (prefix_len == 0) return p;
-    if (M == 0 || (!own.many && batch * kv_heads * ((std::min(max_q, M) * group + 7) / 8) * ((prefix_len + 31) / 32) <= kPrefixSteps))
+    if (prefix_inline(own.many, M, batch, max_q, group, kv_heads, prefix_len))
         p.few = true;
     else
         plan_blocks(&p, M, M, group, kv_heads, prefix_len, bf16);
@@ -136,6 +179,7 @@ struct StateWs {
     size_t m, l, o;
     int pieces;
 };
+size_t state_bytes(size_t records, int hd) { return 2 * a256(records * sizeof(float)) + a256(records * hd * sizeof(float)); }
 struct AttnWs {
     size_t part, total;
     StateWs own, prefix;
@@ -151,7 +195,7 @@ AttnWs attn_ws(const Plan& own, const Plan& pre, int64_t M, int heads, int hd) {
         s.m = w.total;
         s.l = s.m + a256(rows * sizeof(float));
         s.o = s.l + a256(rows * sizeof(float));
-        w.total = s.o + a256(rows * hd * sizeof(float));
+        w.total = s.m + state_bytes(rows, hd);
         return s;
     };
     w.own = take(own.many && (own.splits > 1 || pre.many) ? own.splits : 0);
@@ -347,14 +391,16 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache* cache, const b2s_kv_b
     b2s::KvView v{};
     if (cache_view(cache, &v, "attention_kv_workspace_size")) return 0;
     if (check_shapes(v, batch, M, n_heads, prefix_len, "attention_kv_workspace_size")) return 0;
+    // Enough for either type and for every call of no larger sizes: both rules that lead to states hold for the given sizes if they
+    // hold for any smaller ones, but how many pieces there are does not grow with the sizes.
     const int group = n_heads / v.kv_heads;
-    size_t most = 0;
-    for (int bf16 = 0; bf16 < 2; ++bf16) {  // either type
-        const Plan own = plan_rows(M, batch->batch, batch->max_q, group, v.kv_heads, batch->max_pages << v.page_shift, bf16);
-        const Plan pre = plan_prefix(own, M, batch->batch, batch->max_q, group, v.kv_heads, prefix_len, bf16);
-        most = std::max(most, attn_ws(own, pre, M, n_heads, v.hd).total);
-    }
-    return most;
+    const int64_t rows = M * n_heads;
+    const bool many = std::min<int64_t>(batch->max_q, M) * group > kFewRows;
+    const bool shared = prefix_len > 0 && !prefix_inline(many, M, batch->batch, batch->max_q, group, v.kv_heads, prefix_len);
+    int64_t own = 0, pre = 0;
+    if (many) own = std::max(most_pieces(rows, v.kv_heads, batch->max_pages << v.page_shift), shared ? rows : 0);
+    if (shared) pre = std::max(most_pieces(rows, v.kv_heads, prefix_len), rows);
+    return a256(b2s::kv_attn_part_bytes()) + state_bytes((size_t)own, v.hd) + state_bytes((size_t)pre, v.hd);
 }
 
 int b2s_attention_kv(const b2s_kv_cache* cache, const b2s_kv_batch* batch, int32_t type, const void* q, int64_t ldq,

@@ -225,3 +225,30 @@ def test_a_bad_row_range_in_the_middle_touches_no_sequence_before_it(b2s, prefix
             good[int(start[at - 1]):int(start[at + 1])] = False
             assert bool(((o[:c.rows].double() - ref).abs() <= tol)[good].all())
             assert bool((o[:c.rows][~good] == 7).all() and (o[c.rows:] == 7).all())
+
+
+def workspace(M, batch, max_q, max_pages, prefix, heads, hkv, hd, ps):
+    c = cache_struct(n_kv_heads=hkv, head_dim=hd, page_size=ps)
+    b = batch_struct(batch=batch, max_q=max_q, max_pages=max_pages, ld_pages=max_pages)
+    return kv._bind().b2s_attention_kv_workspace_size(C.byref(c), C.byref(b), M, heads, prefix)
+
+
+def test_the_workspace_of_the_largest_call_is_enough_for_smaller_ones(b2s):
+    """Sized once for the largest shapes it serves every call of no larger ones, also those that cut their keys."""
+    big = workspace(8 * 512, 8, 512, 128, 0, 20, 5, 128, 64)
+    for M, batch, max_q in ((100, 1, 100), (900, 3, 300), (1152, 4, 288), (1, 1, 1), (512, 1, 512)):
+        assert 0 < workspace(M, batch, max_q, 128, 0, 20, 5, 128, 64) <= big
+    g = np.random.default_rng(3)
+
+    def log(hi):
+        return int(np.exp(g.uniform(0, np.log(hi)))) if hi > 1 else hi
+
+    for _ in range(400):
+        hkv = log(16)
+        fixed = (hkv * log(12), hkv, 16 * int(g.integers(1, 9)), 1 << int(g.integers(4, 11)))
+        M, batch, max_q, pages, prefix = log(20000), log(3000), log(20000), log(4000), int(g.integers(0, 2)) * log(200000)
+        size = workspace(M, batch, max_q, pages, prefix, *fixed)
+        assert size > 0 and size % 256 == 0
+        for _ in range(12):
+            less = (log(M), log(batch), log(max_q), log(pages), log(prefix) * int(g.integers(0, 2)))
+            assert workspace(*less, *fixed) <= size, (less, (M, batch, max_q, pages, prefix), fixed)
