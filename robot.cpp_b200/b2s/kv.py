@@ -150,7 +150,7 @@ class Batch:
         dev = _device()
         if pages.get_device() != dev:
             raise ValueError(f"pages must be on the current CUDA device, it is on {pages.device}")
-        self.q_start, self.kv_len, self.pages, self.max_q = q_start, kv_len, pages, int(max_q)
+        self.q_start, self.kv_len, self.pages, self.max_q, self.device = q_start, kv_len, pages, int(max_q), dev
         self.struct = BatchStruct(b, self.max_q, _ints(q_start, torch.int32, (b + 1,), "q_start", dev),
                                   _ints(kv_len, torch.int32, (b,), "kv_len", dev), pages.data_ptr(), pages.shape[1],
                                   pages.stride(0) if b > 1 else pages.shape[1])
@@ -204,21 +204,21 @@ def attention_workspace_size(cache: Cache, batch: Batch, M: int, n_heads: int, p
     return int(_bind().b2s_attention_kv_workspace_size(cache.ref, batch.ref, M, n_heads, prefix_len))
 
 
-def _qo(cache, q, o, n_heads, workspace, dev):
+def _qo(cache, batch, q, o, n_heads, workspace, dev):
     width = n_heads * cache.head_dim
     ty, M, pq, ldq = _rows(q, width, "q", dev)
     _, Mo, po, ldo = _rows(o, width, "o", dev, ty)
     if Mo != M:
         raise ValueError("q and o must have the same rows")
-    if cache.device != dev or workspace.get_device() != dev or not workspace.is_contiguous():
-        raise ValueError("the cache and a contiguous workspace must be on the current CUDA device")
+    if cache.device != dev or batch.device != dev or workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("the cache, the batch and a contiguous workspace must be on the current CUDA device")
     return ty, M, pq, ldq, po, ldo
 
 
 def attention(cache: Cache, batch: Batch, q, n_heads: int, scale: float, causal: bool, o, workspace, stream=None) -> None:
     """o = softmax(scale q K^T) V of each sequence's query rows over its cached tokens (its last tokens, if causal)."""
     dev = _device()
-    ty, M, pq, ldq, po, ldo = _qo(cache, q, o, n_heads, workspace, dev)
+    ty, M, pq, ldq, po, ldo = _qo(cache, batch, q, o, n_heads, workspace, dev)
     check(_bind().b2s_attention_kv(cache.ref, batch.ref, ty, pq, ldq, M, n_heads, scale, int(bool(causal)), po, ldo,
                                    workspace.data_ptr(), workspace.nbytes, _stream(stream, dev)))
 
@@ -227,7 +227,7 @@ def attention_prefix(cache: Cache, batch: Batch, prefix_pages, prefix_len: int, 
                      causal: bool, o, workspace, stream=None) -> None:
     """attention() with prefix_len tokens in prefix_pages [pages] int32 in front of every sequence."""
     dev = _device()
-    ty, M, pq, ldq, po, ldo = _qo(cache, q, o, n_heads, workspace, dev)
+    ty, M, pq, ldq, po, ldo = _qo(cache, batch, q, o, n_heads, workspace, dev)
     if prefix_pages.dim() != 1 or prefix_pages.shape[0] * cache.page_size < prefix_len:
         raise ValueError(f"prefix_pages must hold the pages of {prefix_len} tokens")
     pp = _ints(prefix_pages, torch.int32, prefix_pages.shape, "prefix_pages", dev)

@@ -252,3 +252,48 @@ def test_the_workspace_of_the_largest_call_is_enough_for_smaller_ones(b2s):
         for _ in range(12):
             less = (log(M), log(batch), log(max_q), log(pages), log(prefix) * int(g.integers(0, 2)))
             assert workspace(*less, *fixed) <= size, (less, (M, batch, max_q, pages, prefix), fixed)
+
+
+class Elsewhere:
+    """A tensor on a device of the given index, as far as the binding looks at one."""
+
+    def __init__(self, shape, dtype, device):
+        self.shape, self.dtype, self.device, self.index = torch.Size(shape), dtype, f"cuda:{device}", device
+        self.nbytes = 1 << 40
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i=None):
+        s = [1]
+        for n in self.shape[:0:-1]:
+            s.insert(0, s[0] * n)
+        return tuple(s) if i is None else s[i]
+
+    def get_device(self):
+        return self.index
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return P
+
+
+def test_a_batch_of_another_device_is_refused(b2s, monkeypatch):
+    """A batch built under one device and used under another: its pointers are not passed on."""
+    monkeypatch.setattr(kv, "_raw_stream", lambda dev: 0)
+
+    def on(device):
+        monkeypatch.setattr(kv, "_device", lambda: device)
+        i32 = torch.int32
+        cache = kv.Cache(*[Elsewhere((4, 2, 16, 64), I8, device) for _ in range(2)], *[Elsewhere((4, 2, 16), F32, device) for _ in range(2)])
+        batch = kv.Batch(Elsewhere((3,), i32, device), Elsewhere((2,), i32, device), Elsewhere((2, 2), i32, device), 1)
+        return cache, batch, Elsewhere((2, 256), F32, device), Elsewhere((1,), torch.uint8, device), Elsewhere((2,), i32, device)
+
+    _, batch, *_ = on(0)
+    cache, _, q, ws, pages = on(1)
+    with pytest.raises(ValueError, match="batch"):
+        kv.attention(cache, batch, q, 4, 1.0, True, q, ws)
+    with pytest.raises(ValueError, match="batch"):
+        kv.attention_prefix(cache, batch, pages, 20, q, 4, 1.0, True, q, ws)
