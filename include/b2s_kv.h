@@ -60,7 +60,7 @@ typedef struct b2s_kv_batch {
  * first, or, with interleaved != 0, dealt to the axes in turn, passing over those that have their share. The angle is
  * formed and reduced in double precision, its cosine and sine are fp32 (within 1.5 * 2^-24), and the result is rounded
  * once to `type`. One axis is b2s_rope_neox to those roundings. y may be x (other overlaps are not allowed); M = 0 is
- * allowed; head_dim is even and at most 256; any row alignment that the type allows. */
+ * allowed; head_dim is even and at most 256, a row has fewer than 2^32 - 512 values; any row alignment that the type allows. */
 int b2s_rope_axes(int32_t type, const void *x, int64_t ldx, int64_t M, int n_heads, int head_dim, const int32_t *pos,
                   int64_t ldpos, int n_axes, const int32_t *sections, int interleaved, float theta_base, void *y,
                   int64_t ldy, void *stream);

@@ -314,9 +314,9 @@ int b2s_rope_axes(int32_t type, const void* x, int64_t ldx, int64_t M, int n_hea
     if (!sections || (M > 0 && (!x || !y || !pos)))
         return fail(B2S_ERR_INVALID_ARG, "rope_axes: x, y, pos and sections must be non-NULL");
     if (M < 0 || n_heads <= 0 || head_dim <= 0 || head_dim % 2) return fail(B2S_ERR_INVALID_ARG, "rope_axes: bad shape");
-    if (head_dim > 256 || M > kMaxInt / n_heads)
-        return fail(B2S_ERR_UNSUPPORTED, "rope_axes: head_dim up to 256 and M x n_heads below 2^31");
     const int64_t width = (int64_t)n_heads * head_dim;
+    if (head_dim > 256 || M > kMaxInt / n_heads || width / 2 > kMaxInt - 256)  // a row's pairs are counted in 32 bits, 256 a step
+        return fail(B2S_ERR_UNSUPPORTED, "rope_axes: head_dim up to 256, M x n_heads and a row's pairs below 2^31");
     if (ldx < width || ldy < width) return fail(B2S_ERR_INVALID_ARG, "rope_axes: row stride below n_heads * head_dim");
     if (!aligned(x, size_of(type)) || !aligned(y, size_of(type)))
         return fail(B2S_ERR_UNSUPPORTED, "rope_axes: x or y is not aligned to its type");

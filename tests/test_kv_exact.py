@@ -297,3 +297,11 @@ def test_a_batch_of_another_device_is_refused(b2s, monkeypatch):
         kv.attention(cache, batch, q, 4, 1.0, True, q, ws)
     with pytest.raises(ValueError, match="batch"):
         kv.attention_prefix(cache, batch, pages, 20, q, 4, 1.0, True, q, ws)
+
+
+@pytest.mark.parametrize("heads,hd", [(2 ** 24, 256), (2 ** 25, 128), (2 ** 30, 4), (2 ** 30 - 64, 4)])
+def test_rope_axes_refuses_rows_past_32_bits(b2s, heads, hd):
+    """A row of nearly 2^31 pairs or more: its pairs are counted in 32 bits."""
+    width = heads * hd
+    assert kv._bind().b2s_rope_axes(30, P, width, 1, heads, hd, P, 1, 1, (C.c_int32 * 1)(hd // 2), 0, 1e4, 2 * P, width, None) == UNSUPPORTED
+    assert "2^31" in b2s.last_error()
