@@ -227,6 +227,7 @@ int attention(const char* op, const b2s_kv_cache* cache, const b2s_kv_batch* bat
     const int64_t width = (int64_t)n_heads * v.hd;
     if ((rc = check_rows(q, M, ldq, width, type, op, "q"))) return rc;
     if ((rc = check_rows(o, M, ldo, width, type, op, "o"))) return rc;
+    if (M > 1 && q == o && ldq != ldo) return fail(B2S_ERR_INVALID_ARG, "%s: in place needs ldq == ldo", op);
     if (!std::isfinite(scale * 2.0f)) return fail(B2S_ERR_INVALID_ARG, "%s: scale is not finite or too large", op);
     if (batch->batch > 0) {
         if (!batch->q_start || !batch->kv_len) return fail(B2S_ERR_INVALID_ARG, "%s: q_start or kv_len is NULL", op);

@@ -305,3 +305,12 @@ def test_rope_axes_refuses_rows_past_32_bits(b2s, heads, hd):
     width = heads * hd
     assert kv._bind().b2s_rope_axes(30, P, width, 1, heads, hd, P, 1, 1, (C.c_int32 * 1)(hd // 2), 0, 1e4, 2 * P, width, None) == UNSUPPORTED
     assert "2^31" in b2s.last_error()
+
+
+def test_attention_in_place_needs_one_stride(b2s):
+    """o may be q; with another row stride rows would be written over queries that are still to be read."""
+    L, c, b = kv._bind(), cache_struct(), batch_struct()
+    args = (0, P, 2560, 4, 20, 0.1, 1, P, 2564, 2 * P, 1 << 40, None)
+    assert L.b2s_attention_kv(C.byref(c), C.byref(b), *args) == INVALID
+    assert "in place" in b2s.last_error()
+    assert L.b2s_attention_kv_prefix(C.byref(c), C.byref(b), P, 100, *args) == INVALID
