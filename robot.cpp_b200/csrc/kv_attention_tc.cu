@@ -304,7 +304,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
     Misc* ms = reinterpret_cast<Misc*>(raw + kKeys * HDP);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // warp: the same in every lane
     griddep_wait();
-    griddep_launch();
 
     // ---- which sequence, row block, head and share of the keys: later row blocks, which see more keys, go first
     const int h = blockIdx.x % a.c.kv_heads;
@@ -377,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const KvAt
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    griddep_launch();  // not before: the next grid may take tensor memory first and then wait for this one, which waits for that memory
     const uint32_t tmem = __shfl_sync(0xffffffffu, ms->tmem, 0);
     const int b = (int)ms->found[0], row0 = (int)ms->found[1] * kBlkRows;
     const Rows sq = ms->seq;

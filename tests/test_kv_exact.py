@@ -14,6 +14,7 @@ An output is then one rounding of what lies within that: o is between the rounde
 """
 import ctypes as C
 import math
+import os
 
 import numpy as np
 import pytest
@@ -314,3 +315,16 @@ def test_attention_in_place_needs_one_stride(b2s):
     assert L.b2s_attention_kv(C.byref(c), C.byref(b), *args) == INVALID
     assert "in place" in b2s.last_error()
     assert L.b2s_attention_kv_prefix(C.byref(c), C.byref(b), P, 100, *args) == INVALID
+
+
+def test_no_grid_is_let_in_before_tensor_memory_is_allocated():
+    """A kernel that lets the next grid start first may find its tensor memory taken by a block of that grid, which waits for it."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "robot.cpp_b200", "csrc")
+    seen = 0
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith(".cu"):
+            for kernel in open(os.path.join(csrc, name)).read().split("__global__")[1:]:
+                if "tmem_alloc(" in kernel:
+                    seen += 1
+                    assert "griddep_launch()" not in kernel[:kernel.index("tmem_alloc(")], name
+    assert seen >= 4
