@@ -22,7 +22,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from b2s import kv  # noqa: E402
-from test_kv import BF16, E4M3, F32, I8, INVALID, TOP, U, UNSUPPORTED, Case, P, batch_struct, cache_struct, gen, gpu, ok, randn  # noqa: E402
+from test_kv import BF16, E4M3, F32, HALF, I8, INVALID, U, UNSUPPORTED, Case, P, batch_struct, cache_struct, gen, gpu, ok, randn, rope_ref  # noqa: E402
 
 
 def interval(c, products):
@@ -328,3 +328,85 @@ def test_no_grid_is_let_in_before_tensor_memory_is_allocated():
                     seen += 1
                     assert "griddep_launch()" not in kernel[:kernel.index("tmem_alloc(")], name
     assert seen >= 4
+
+
+@gpu
+@pytest.mark.parametrize("new,keys,heads,hkv,hd,prefix", MANY + [
+    ([1], [1], 1, 1, 16, 0), ([1], [4000], 2, 1, 128, 0), ([1], [3000], 4, 4, 64, 5000), ([3, 5, 1], [300, 40, 1000], 32, 4, 64, 0),
+    ([65], [4096], 2, 1, 32, 0), ([129], [1301], 3, 3, 96, 77), ([96, 1, 96], [2049, 2049, 127], 6, 1, 128, 0), ([9], [600], 20, 5, 128, 0),
+    ([1] * 300, [1 + 7 * (i % 40) for i in range(300)], 6, 3, 64, 0), ([2, 1] * 100, [40, 3] * 100, 8, 4, 80, 33)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,code", [(F32, I8), (BF16, E4M3)])
+def test_every_key_counts_once(b2s, new, keys, heads, hkv, hd, prefix, causal, dtype, code):
+    """Queries of zero give every visible key the same weight. Token j's value is a whole number in column j % head_dim and zero in
+    the others: sums and counts are exact, and one key too few or too many changes a column by more than 2^-10 of it and every other
+    one by 1 / n, where fp32 outputs are held to 2^-13 at the longest."""
+    c = Case(141, new, keys, heads, hkv, hd, 16, dtype, code, causal, prefix, extra_rows=2)
+    c.q.zero_()
+    c.cache.k_scale.fill_(1.0)
+    c.cache.v_scale.fill_(1.0)
+    c.cache.v.view(torch.uint8).zero_()
+    for pages, n, first in [(c.prefix_pages, prefix, 0)] + [(c.pages[b], n, prefix) for b, n in enumerate(keys)]:
+        if n:
+            j = torch.arange(n, device="cuda")
+            value = (1 + (first + j) // hd % 8).to(F32)  # 1 .. 8: also exact in e4m3
+            row = torch.zeros(n, hkv, hd, device="cuda")
+            row[j, :, (first + j) % hd] = value[:, None]
+            c.cache.v.view(torch.uint8)[pages[j // 16].long(), :, j % 16] = row.to(c.cache.v.dtype).view(torch.uint8)
+    o = c.run()
+    ok(b2s)
+    inside(c, o, 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,heads,hd,sections,inter", [
+    (40, 5, 128, [24, 20, 20], True), (33, 3, 72, [36], False), (700, 2, 32, [5, 11], False), (9, 2, 256, [0, 100, 28], True)])
+def test_rope_axes_within_its_roundings(b2s, dtype, M, heads, hd, sections, inter):
+    """Each row against its own positions' bound: the angle is a double, 2^-51 of the position in radians; cosine and sine within 1.5 * 2^-24
+    (read off rows that are zero in one half), two products and a sum of 2^-24 each, one rounding to the type."""
+    g = gen(M + hd)
+    pos = (10.0 ** (9 * torch.rand((M, len(sections)), generator=g, device="cuda"))).to(torch.int32)
+    x = randn(g, M, heads * hd, dtype=dtype)
+    ref, mag = rope_ref(x, heads, hd, pos, sections, 500000.0, inter)
+    y = torch.empty_like(x)
+    kv.rope_axes(x, heads, hd, pos, sections, 500000.0, y, inter)
+    ok(b2s)
+    angle = pos.double().amax(1, keepdim=True) * 2.0 ** -51
+    assert bool(((y.double() - ref).abs() <= (4 * U + angle) * mag + HALF[dtype] * ref.abs()).all())
+    if dtype == F32:
+        x.view(M, heads, 2, hd // 2)[:, :, 1] = 0
+        x.view(M, heads, 2, hd // 2)[:, :, 0] = 1
+        ref, _ = rope_ref(x, heads, hd, pos, sections, 500000.0, inter)
+        kv.rope_axes(x, heads, hd, pos, sections, 500000.0, y, inter)
+        ok(b2s)
+        assert bool(((y.double() - ref).abs() <= 1.5 * U + angle).all())
+
+
+@gpu
+def test_scale_offsets_pass_32_bits(b2s):
+    """Scales whose byte offsets, and codes whose offsets, lie past 2^31 and 2^32."""
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB of device memory")
+    pages, ps = 2 ** 19 + 2 ** 14, 1024  # 5.5e8 tokens: 8.9e9 code bytes and 2.2e9 scale bytes each for keys and values
+    cache = kv.Cache.empty(pages, 1, ps, 16)
+    for t in (cache.k, cache.v, cache.k_scale, cache.v_scale):
+        t.zero_()
+    g, n = gen(61), 1500
+    slots = torch.arange(n, device="cuda") + (pages - 2) * ps
+    k, v = randn(g, n, 16), randn(g, n, 16)
+    kv.write(cache, k, v, slots)
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    kv.read(cache, slots, ko, vo)
+    ok(b2s)
+    assert float((ko - k).abs().max()) <= float(k.abs().max()) * 0.51 / 127 and float((vo - v).abs().max()) <= float(v.abs().max()) * 0.51 / 127
+    table = torch.tensor([[pages - 2, pages - 1]], dtype=torch.int32, device="cuda")
+    for rows in (1, 100):
+        q, o = torch.zeros(rows, 64, device="cuda"), torch.empty(rows, 64, device="cuda")
+        batch = kv.Batch(torch.tensor([0, rows], dtype=torch.int32, device="cuda"),
+                         torch.tensor([n], dtype=torch.int32, device="cuda"), table, rows)
+        ws = torch.empty(kv.attention_workspace_size(cache, batch, rows, 4), dtype=torch.uint8, device="cuda")
+        kv.attention(cache, batch, q, 4, 0.1, False, o, ws)
+        ok(b2s)
+        ref = vo.double().mean(0).repeat(rows, 4)  # equal weights
+        assert float((o.double() - ref).abs().max()) <= ((16 + n / 8) * 2.0 ** -23 + 2.0 ** -21) * float(vo.double().abs().mean(0).max())
