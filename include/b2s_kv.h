@@ -91,10 +91,12 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache *cache, const b2s_kv_b
  * tokens j <= kv_len - n + i, else all. A row that sees nothing is written as zeros; rows of o outside
  * [q_start[0], q_start[batch]) are left as they were. o may be q, with the same row stride (other overlaps are not allowed). scale is finite and below 2^127.
  * Scores, softmax and sums are fp32, products run on the tensor cores, where the 8-bit codes are exact. fp32 queries
- * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or of its row's largest one: 2^-39 where few
+ * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or of its row's largest one: 2^-38 where few
  * rows share a key/value head; where many do, 2^-33 for queries and 2^-32 for probabilities times their value scales), or,
- * queries of few rows on int8 codes, as integers of 24 bits under the row's largest element; bf16 queries likewise or exactly,
- * their probabilities as fp32 ones. A query head with an infinity or a NaN is NaN; no other one is. */
+ * queries of few rows on int8 codes, as integers of 24 bits under the row's largest element or 2^-100, if that is larger; bf16
+ * queries likewise or exactly, their probabilities as fp32 ones. Where many rows share a head, the tensor cores cut sums off
+ * below their last bit: about 2^-31 for each key that one block takes (5e-6 of an output over 8192 keys).
+ * A query head with an infinity or a NaN is NaN; no other one is, as long as scores are within fp32's range. */
 int b2s_attention_kv(const b2s_kv_cache *cache, const b2s_kv_batch *batch, int32_t type, const void *q, int64_t ldq,
                      int64_t M, int n_heads, float scale, int causal, void *o, int64_t ldo, void *workspace,
                      size_t workspace_bytes, void *stream);

@@ -77,8 +77,8 @@ int cache_view(const b2s_kv_cache* c, b2s::KvView* v, const char* op) {
 // Which kernels take the rows of a call, decided from sizes that the host has. Sequences with at most kFewRows rows a
 // key/value head go to the warp-level kernel, which reads their keys once per eight rows; the others to the tensor-core
 // kernel, which reads them once per 128. Five heads of 128, int8, us with the first and with the second kernel: 16 sequences
-// of 2000 keys, 20 rows 41 and 55 (bf16 40 and 44), 32 rows 49 and 56 (47 and 45), 48 rows 66 and 57 (64 and 45), 64 rows 82 and
-// 57 (80 and 45); one sequence, 32 rows 18.2 and 18.5 (17.2 and 15.5), 64 rows 22.6 and 19.4 (21.0 and 15.9).
+// of 2000 keys, 20 rows 40 and 60 (bf16 39 and 56), 32 rows 48 and 62 (46 and 56), 48 rows 64 and 62 (63 and 58), 64 rows 81 and
+// 65 (79 and 59); one sequence, 32 rows 18.5 and 20.0 (17.0 and 18.1), 64 rows 21.6 and 20.8 (20.2 and 18.9).
 constexpr int kFewRows = 32;
 struct Plan {
     bool few, many, pair;  // pair: blocks of 256 rows
@@ -87,9 +87,11 @@ struct Plan {
 // The tensor-core kernel's part of a plan for M tokens of up to max_q a sequence over `keys` keys: blocks of 128 or (bf16) 256
 // rows, and into how many shares the keys are cut where that gives less than a wave of blocks. The least estimate is taken, in
 // half tiles' time: waves x (a block's tiles of 128 keys, 2 each or 3 for 256 rows, + 8 or 12 to start and end it), + 6 for the
-// join. bf16, five heads, us with blocks of 128 and of 256 rows: one sequence of 256 rows on 2000 keys 19 and 27, 8 of 260 on
-// 2000 keys 45 and 76, 2 of 2048 on 4096 keys 144 and 119, 8 of 512 on 128 keys 23 and 18. fp32, whole keys and cut ones: 260
-// rows on 8192 keys 175 and 40, 512 on 2000 keys 54 and 27, 4096 rows of one head on 4096 keys 94 and 41.
+// join. bf16, five heads, us with blocks of 128 and of 256 rows: one sequence of 256 rows on 2000 keys 22 and 28, 8 of 260 on
+// 2000 keys 58 and 83, 2 of 2048 on 4096 keys 173 and 141, 8 of 512 on 128 keys 26 and 19. fp32, whole keys and cut ones: 260
+// rows on 8192 keys 183 and 44, 512 on 2000 keys 59 and 29, 4096 rows of one head on 4096 keys 100 and 45. The host knows the
+// table's width, not the lengths in it: 4 sequences of 100 fp32 tokens take 17 us behind a table of 2 pages of 64 and 45 behind
+// one of 128, whose keys are cut for nothing.
 constexpr int kMaxSplits = 16, kWave = 148;
 // Numbers of tiles that are planned for: each up to 64, then eight an octave, so that most_pieces can go through them all.
 int64_t tile_step(int64_t tiles) {
@@ -158,8 +160,8 @@ Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads,
 
 // A shared prefix goes through the tensor-core kernel, once for all rows, unless few rows make it cheaper to let every
 // sequence read it with its own tokens (from L2): up to kPrefixSteps steps of 32 keys and eight rows. One pass then takes the
-// place of three. 20 heads on 5, int8, us with one pass and with three: 16 rows on 545 shared tokens (1440 steps) 21.5 and 25.1,
-// 32 on 1600 (8000) 30.2 and 31.0, 64 on 800 (8000) 32.4 and 30.2, 64 on 1600 (16000) 43.9 and 32.4.
+// place of three. 20 heads on 5, int8, us with one pass and with three: 16 rows on 545 shared tokens (1440 steps) 21.3 and 25.3,
+// 32 on 1600 (8000) 29.6 and 30.7, 64 on 800 (8000) 31.8 and 30.4, 64 on 1600 (16000) 43.1 and 32.5.
 constexpr int64_t kPrefixSteps = 8192;
 bool prefix_inline(bool own_many, int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t prefix_len) {
     return M == 0 || (!own_many && batch * kv_heads * ((std::min(max_q, M) * group + 7) / 8) * ((prefix_len + 31) / 32) <= kPrefixSteps);

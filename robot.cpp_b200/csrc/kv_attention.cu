@@ -24,8 +24,8 @@
 // by a range's border leaves partial results that kv_attention_join_kernel puts together: the order is fixed by the
 // lengths alone, so results do not change from run to run. Short units are not cut, and many short ones go to a warp each.
 //
-// Measured, 20 heads on 5 of 128, one fp32 row a sequence, int8: 64 sequences of 1024..8192 tokens 97 us, 4.3 TB/s of a copy's
-// 6.5; 64 of 8192 tokens 135 us, 5.2 TB/s (e4m3 and bf16 127 us, 5.4); one of 32768 29 us; one of 317 9.8 us. What bounds it is
+// Measured, 20 heads on 5 of 128, one fp32 row a sequence, int8: 64 sequences of 1024..8192 tokens 95 us, 4.4 TB/s of a copy's
+// 6.5; 64 of 8192 tokens 132 us, 5.2 TB/s (e4m3 and bf16 125-133 us); one of 32768 29 us; one of 317 9.7-11 us. What bounds it is
 // the warps' own work between two tiles (issue slots 53% busy, memory 53%), then starting and joining units.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -277,7 +277,7 @@ kv_write_kernel(KvView c, const T* __restrict__ k, int64_t ldk, const T* __restr
     const float a = bad ? 1.0f : fmaxf(__uint_as_float(mine), 0x1p-100f);
     const float up = bad ? 0.0f : __fdiv_rn(top, a);
     if (lane < kWriteSteps<LANES> && f0 + lane * step < heads) {
-        // a / top, correctly rounded: the quotient by the rounded reciprocal, corrected once by its exact remainder
+        // a / top, correctly rounded: the quotient by the rounded reciprocal, corrected once by its exact remainder (Markstein's theorem)
         const float q0 = __fmul_rn(a, by_top), quotient = __fmaf_rn(__fmaf_rn(-q0, top, a), by_top, q0);
         const int f = f0 + lane * step;
         (f < c.kv_heads ? c.ks : c.vs)[row_of(f)] = bad ? __int_as_float(0x7fc00000) : quotient;
