@@ -89,7 +89,8 @@ size_t b2s_attention_kv_workspace_size(const b2s_kv_cache *cache, const b2s_kv_b
 /* o = softmax(scale * q K^T) V of every sequence's query rows over its cached tokens; q and o [M][n_heads * head_dim]
  * of `type`, query head h reads key/value head h / (n_heads / n_kv_heads). With causal != 0 query row i of n sees the
  * tokens j <= kv_len - n + i, else all. A row that sees nothing is written as zeros; rows of o outside
- * [q_start[0], q_start[batch]) are left as they were. o may be q, with the same row stride (other overlaps are not allowed). scale is finite and below 2^127.
+ * [q_start[0], q_start[batch]) are left as they were. o may be q, with the same row stride (other overlaps are
+ * not allowed). scale is finite and below 2^127.
  * Scores, softmax and sums are fp32, products run on the tensor cores, where the 8-bit codes are exact. fp32 queries
  * and probabilities are taken as two fp16 parts (error 2^-22 of the element, or of its row's largest one: 2^-38 where few
  * rows share a key/value head; where many do, 2^-33 for queries and 2^-32 for probabilities times their value scales), or,

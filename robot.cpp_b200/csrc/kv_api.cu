@@ -93,59 +93,53 @@ struct Plan {
 // table's width, not the lengths in it: 4 sequences of 100 fp32 tokens take 17 us behind a table of 2 pages of 64 and 45 behind
 // one of 128, whose keys are cut for nothing.
 constexpr int kMaxSplits = 16, kWave = 148;
-// Numbers of tiles that are planned for: each up to 64, then eight an octave, so that most_pieces can go through them all.
-int64_t tile_step(int64_t tiles) {
-    int64_t step = 1;
-    while (tiles / step >= (step == 1 ? 64 : 16)) step *= step == 1 ? 8 : 2;
-    return step;
-}
-int64_t planned_tiles(int64_t keys) {
-    const int64_t tiles = std::max<int64_t>(1, (keys + 127) / 128), step = tile_step(tiles);
-    return (tiles + step - 1) / step * step;
-}
-// The number of shares of the least estimate for `units` blocks' worth of whole rows, and that estimate.
-int best_splits(int64_t units, int64_t tiles, int pair, int64_t* least) {
-    int best = 1;
-    for (int s = 1; s <= kMaxSplits && s <= tiles && (s == 1 || units < kWave); ++s) {
-        const int64_t cost = (units * s + kWave - 1) / kWave * ((tiles + s - 1) / s * (2 + pair) + 8 + 4 * pair) + (s > 1 ? 6 : 0);
-        if (s == 1 || cost < *least) {
-            *least = cost;
-            best = s;
-        }
-    }
-    return best;
-}
+int64_t waves(int64_t units, int s) { return (units * s + kWave - 1) / kWave; }
+constexpr int tile_cost(int pair) { return 2 + pair; }
+constexpr int block_cost(int pair) { return 8 + 4 * pair; }
+constexpr int kJoinCost = 6;
 void plan_blocks(Plan* p, int64_t M, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
     p->many = true;
-    const int64_t seqs = std::max<int64_t>(1, (M + max_q - 1) / max_q), tiles = planned_tiles(keys);
+    const int64_t seqs = (M + max_q - 1) / max_q, tiles = std::max<int64_t>(1, (keys + 127) / 128);
     int64_t best = -1;
     for (int pair = 0; pair <= (bf16 ? 1 : 0); ++pair) {
-        int64_t cost = 0;
-        const int s = best_splits(seqs * ((max_q * group + 128 * (1 + pair) - 1) / (128 * (1 + pair))) * kv_heads, tiles, pair, &cost);
-        if (best < 0 || cost < best) {
-            best = cost;
-            p->pair = pair != 0;
-            p->splits = s;
-        }
-    }
-}
-// The most pieces (of a row and head) that cut keys leave in any call of up to `rows` rows x heads over up to `keys` keys: calls of
-// fewer rows or keys may be cut where the largest is not. M rows in blocks of 128 or 256 a sequence and key/value head are at most
-// that many rows x heads for each unit.
-int64_t most_pieces(int64_t rows, int kv_heads, int64_t keys) {
-    int64_t most = 0;
-    const int64_t last = planned_tiles(keys);
-    for (int64_t units = (kWave - 1) / kv_heads * kv_heads; units > 0; units -= kv_heads) {
-        for (int pair = 0; pair < 2; ++pair) {
-            const int64_t held = std::min(rows, units * 128 * (1 + pair));
-            if (held * kMaxSplits <= most) continue;
-            for (int64_t tiles = 2; tiles <= last; tiles += tile_step(tiles)) {
-                int64_t cost = 0;
-                const int s = best_splits(units, tiles, pair, &cost);
-                if (s > 1) most = std::max(most, held * s);
+        const int64_t units = std::max<int64_t>(1, seqs) * ((max_q * group + 128 * (1 + pair) - 1) / (128 * (1 + pair))) * kv_heads;
+        for (int s = 1; s <= kMaxSplits && s <= tiles && (s == 1 || units < kWave); ++s) {
+            const int64_t cost = waves(units, s) * ((tiles + s - 1) / s * tile_cost(pair) + block_cost(pair)) + (s > 1 ? kJoinCost : 0);
+            if (best < 0 || cost < best) {
+                best = cost;
+                p->pair = pair != 0;
+                p->splits = s;
             }
         }
     }
+}
+// Whether a call of `units` blocks over some number of tiles up to `most` may be cut into s shares: that has to cost less than
+// every smaller number, s1, of them, tiles / s tiles a share and without rounding up against (tiles + s1 - 1) / s1. Both sides are
+// linear in the tiles, so where it is false for the fewest and for the most tiles it is false between them.
+bool may_be_cut(int64_t units, int s, int64_t most, int pair) {
+    const int64_t w = waves(units, s), tile = tile_cost(pair), block = block_cost(pair);
+    for (int s1 = 1; s1 < s; ++s1) {
+        const int64_t w1 = waves(units, s1);
+        auto less = [&](int64_t tiles) {  // times s s1
+            return s1 * (w * (tile * tiles + block * s) + kJoinCost * s) <
+                   s * (w1 * (tile * (tiles + s1 - 1) + block * s1) + (s1 > 1 ? kJoinCost * s1 : 0));
+        };
+        if (!less(s) && !less(most)) return false;
+    }
+    return true;
+}
+// A bound of the pieces (of a row and head) that cut keys leave in any call of up to `rows` rows x heads over up to `keys` keys:
+// calls of fewer rows or keys may be cut where the largest is not. A call of `units` < kWave blocks has at most that many times 128
+// or 256 rows x heads.
+int64_t most_pieces(int64_t rows, int kv_heads, int64_t keys) {
+    int64_t most = 0;
+    const int64_t tiles = (keys + 127) / 128;
+    for (int64_t units = kv_heads; units < kWave; units += kv_heads)
+        for (int pair = 0; pair < 2; ++pair) {
+            const int64_t held = std::min(rows, units * 128 * (1 + pair));
+            for (int s = (int)std::min<int64_t>(kMaxSplits, tiles); s > 1 && held * s > most; --s)
+                if (may_be_cut(units, s, tiles, pair)) most = held * s;
+        }
     return most;
 }
 Plan plan_rows(int64_t M, int64_t batch, int64_t max_q, int group, int kv_heads, int64_t keys, bool bf16) {
